@@ -28,6 +28,29 @@ _c_i64 = ctypes.c_int64
 _c_dbl = ctypes.c_double
 _c_ptr = ctypes.c_void_p
 
+
+class PagedKVStruct(ctypes.Structure):
+    """``ako_b200_paged_kv`` of include/ako_b200.h."""
+
+    _fields_ = [
+        *((n, _c_ptr) for n in ("k", "v", "k_scale", "v_scale")),
+        *((f"{t}_stride_{a}", _c_i64) for t in ("k", "v", "ks", "vs") for a in ("page", "head", "slot")),
+        *((n, _c_i64) for n in ("num_pages", "kv_heads", "page_size", "head_dim", "dtype")),
+    ]
+
+
+class PagedBatchStruct(ctypes.Structure):
+    """``ako_b200_paged_batch`` of include/ako_b200.h."""
+
+    _fields_ = [
+        *((n, _c_ptr) for n in ("page_table", "kv_lens", "cu_seqlens")),
+        *((n, _c_i64) for n in ("page_table_stride", "batch", "max_pages", "max_q_len")),
+    ]
+
+
+_c_kv = ctypes.POINTER(PagedKVStruct)
+_c_seqs = ctypes.POINTER(PagedBatchStruct)
+
 #: Exported symbol -> (restype, argtypes); mirrors include/ako_b200.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ako_b200_abi_version": (_c_int, []),
@@ -67,6 +90,26 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                        ctypes.POINTER(_c_int), ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
                                        ctypes.POINTER(_c_int)]),
     "ako_b200_take_device_status": (_c_int, [ctypes.POINTER(ctypes.c_int)]),
+    "ako_b200_kv_cache_write": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_kv, _c_seqs, _c_i64, _c_i64, _c_int,
+         _c_ptr],
+    ),
+    "ako_b200_kv_cache_read": (
+        _c_int,
+        [_c_kv, _c_seqs, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_int,
+         _c_ptr],
+    ),
+    "ako_b200_paged_attention": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_i64, _c_kv, _c_seqs, _c_i64, _c_i64, _c_i64, _c_dbl, _c_i64, _c_i64,
+         _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_int, _c_ptr],
+    ),
+    "ako_b200_paged_attention_plan": (
+        _c_int,
+        [_c_kv, _c_seqs, _c_i64, _c_i64, _c_i64, _c_int, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
+         ctypes.POINTER(_c_int), ctypes.POINTER(_c_i64)],
+    ),
 }
 
 #: Symbols only the measurement build exports; mirrors include/ako_b200_measure.h.

@@ -1,0 +1,504 @@
+// Writing new tokens into a paged key/value cache and reading sequences back.
+//
+// Both move each value once and compute next to nothing, so both are bound by
+// memory: by HBM where there are megabytes to move, by the chain
+// lengths -> page number -> access where there are few.
+#include <climits>
+
+#include <cuda_fp8.h>
+
+#include "paged.cuh"
+
+namespace ako_b200 {
+
+// ------------------------------------------------------------ argument checks
+namespace {
+
+bool multiple16(int64_t stride, int64_t extent, int es) { return extent <= 1 || ((stride * es) & 15) == 0; }
+
+bool tensor16(const PagedTensor& t, const ako_b200_paged_kv& c, int es) {
+    return aligned16(t.p) && multiple16(t.page, c.num_pages, es) && multiple16(t.head, c.kv_heads, es) &&
+           multiple16(t.slot, c.page_size, es);
+}
+
+}  // namespace
+
+int make_cache(const char* op, const ako_b200_paged_kv* c, int dtype, PagedCache& out, int& cache_es) {
+    if (c == nullptr) return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: cache is a null pointer", op);
+    if (dtype_size(dtype) == 0)
+        return set_error(AKO_B200_ERR_UNSUPPORTED_DTYPE, "%s: unsupported dtype code %d", op, dtype);
+    const bool e4m3 = c->dtype == AKO_B200_E4M3;
+    if (!e4m3 && (c->dtype < 0 || c->dtype > AKO_B200_BF16))
+        return set_error(AKO_B200_ERR_UNSUPPORTED_DTYPE, "%s: unsupported cache dtype code %lld", op,
+                         static_cast<long long>(c->dtype));
+    if (!e4m3 && c->dtype != dtype)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: dtype %d differs from the cache's %lld", op, dtype,
+                         static_cast<long long>(c->dtype));
+    cache_es = e4m3 ? 1 : dtype_size(dtype);
+    if (c->num_pages < 1 || c->num_pages > INT_MAX || c->kv_heads < 1 || c->kv_heads > 65535 || c->page_size < 1 ||
+        c->page_size > INT_MAX)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: num_pages, kv_heads and page_size must be >= 1 (and "
+                                                        "kv_heads <= 65535)", op);
+    const int step = e4m3 ? 16 : 8;
+    if (c->head_dim < step || c->head_dim > 128 || c->head_dim % step != 0)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: head_dim must be a multiple of %d up to 128, got %lld", op,
+                         step, static_cast<long long>(c->head_dim));
+    if (c->k == nullptr || c->v == nullptr)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k or v of the cache is a null pointer", op);
+    if (e4m3 && (c->k_scale == nullptr || c->v_scale == nullptr))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: an e4m3 cache needs k_scale and v_scale", op);
+    out.k = PagedTensor{c->k, c->k_stride_page, c->k_stride_head, c->k_stride_slot};
+    out.v = PagedTensor{c->v, c->v_stride_page, c->v_stride_head, c->v_stride_slot};
+    out.ks = PagedTensor{c->k_scale, c->ks_stride_page, c->ks_stride_head, c->ks_stride_slot};
+    out.vs = PagedTensor{c->v_scale, c->vs_stride_page, c->vs_stride_head, c->vs_stride_slot};
+    if (!e4m3) out.ks.p = out.vs.p = nullptr;
+    if (!tensor16(out.k, *c, cache_es) || !tensor16(out.v, *c, cache_es))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k and v of the cache and their strides must be multiples "
+                                                        "of 16 bytes", op);
+    out.num_pages = static_cast<int>(c->num_pages);
+    out.kv_heads = static_cast<int>(c->kv_heads);
+    out.head_dim = static_cast<int>(c->head_dim);
+    out.page_size = static_cast<int>(c->page_size);
+    out.by_page = FastDiv::make(static_cast<uint32_t>(c->page_size));
+    return AKO_B200_OK;
+}
+
+int make_seqs(const char* op, const ako_b200_paged_batch* b, const PagedCache& c, int64_t tokens, int64_t q_len,
+              PagedSeqs& out) {
+    if (b == nullptr) return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: batch is a null pointer", op);
+    if (b->batch < 0 || b->batch > 65535 || b->max_pages < 0)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: batch must be within 0 .. 65535 and max_pages >= 0", op);
+    if (b->max_pages > 0 && b->max_pages > (INT_MAX - 4096) / c.page_size)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: max_pages * page_size must be < 2^31 - 4096", op);
+    if (tokens < 0 || q_len < 0 || tokens > INT_MAX)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: tokens and q_len must be within 0 .. 2^31 - 1", op);
+    if (b->cu_seqlens == nullptr && (q_len > INT_MAX || b->batch * q_len != tokens))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: without cu_seqlens tokens must be batch * q_len", op);
+    if (b->batch > 0 && (b->kv_lens == nullptr || (b->max_pages > 0 && b->page_table == nullptr)))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: page_table or kv_lens is a null pointer", op);
+    if (b->batch > 1 && b->page_table_stride < b->max_pages)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: page_table_stride %lld is smaller than max_pages", op,
+                         static_cast<long long>(b->page_table_stride));
+    out.table = b->page_table;
+    out.table_stride = b->page_table_stride;
+    out.kv_lens = b->kv_lens;
+    out.cu = b->cu_seqlens;
+    out.batch = static_cast<int>(b->batch);
+    out.q_len = static_cast<int>(q_len);
+    out.tokens = static_cast<int>(tokens);
+    out.max_kv = static_cast<int>(b->max_pages * c.page_size);
+    return AKO_B200_OK;
+}
+
+namespace {
+
+// ------------------------------------------------------------------ e4m3
+// Eight fp32 values as e4m3, to nearest even, saturating (NaN stays NaN).
+__device__ __forceinline__ uint2 to_e4m3(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+}
+
+__device__ __forceinline__ float2 from_e4m3(uint32_t pair) {
+    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3)));
+}
+
+// Exponent of the least power of two s with top / s <= 448 = 1.75 * 2^8, at
+// least -126 (so that s and 1 / s are normal); top is finite and positive.
+__device__ __forceinline__ int scale_exponent(float top) {
+    const uint32_t u = __float_as_uint(top);
+    const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return max(e, -126);
+}
+
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// ------------------------------------------------------------ row accesses
+// Eight elements of T (one 16-byte access for 16-bit types, two for fp32).
+template <typename T>
+struct Row8 {
+    static constexpr int N = 8 * sizeof(T) / 16;
+    uint4 w[N];
+
+    __device__ __forceinline__ void load(const void* base, int64_t at) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(base) + at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = p[i];
+    }
+    __device__ __forceinline__ void store(void* base, int64_t at) const {
+        uint4* p = reinterpret_cast<uint4*>(static_cast<T*>(base) + at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = w[i];
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const T* v = reinterpret_cast<const T*>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
+    }
+    __device__ __forceinline__ void put(const float (&x)[8]) {
+        auto& v = *reinterpret_cast<Packed<T, 8>*>(w);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) put2(v, i, x[i], x[i + 1]);
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+};
+
+constexpr int kThreads = 256;
+
+// Lanes that share a row of head_dim elements, `each` to a lane: a power of
+// two, as its logarithm.
+int lanes_log2(int head_dim, int each) {
+    int l = 0;
+    while ((each << l) < head_dim) ++l;
+    return l;
+}
+
+// Rows per thread: the most that still gives every SM `ctas` CTAs.
+int rows_per_thread(int64_t rows, int rows_per_pass, int most, int ctas) {
+    const int64_t passes = (rows + rows_per_pass - 1) / rows_per_pass;
+    return passes >= static_cast<int64_t>(most) * ctas * sm_count() ? most : 1;
+}
+
+// ------------------------------------------------------------------- write
+struct WriteArgs {
+    const void *k, *v;
+    int64_t kb, ks, kh, vb, vs, vh;
+    PagedCache cache;
+    PagedSeqs seqs;
+    FastDiv heads, q_len;
+    uint32_t rows;  // tokens * kv_heads
+    int lanes_log2;
+};
+
+// Sequence of token `t` under cu_seqlens: the last b with cu[b] <= t, or 0.
+// All lanes of a warp call it: they search together for their least token,
+// 32 entries at a time, then each walks on to its own.
+__device__ __forceinline__ int find_sequence(const int* cu, int batch, int t) {
+    const int least = __reduce_min_sync(0xffffffffu, t);
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    int lo = 0, hi = batch;  // the answer for `least` lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5;
+        const int at = lo + step * (lane + 1);
+        // cu is not decreasing, so these are the first lanes
+        const int n = __popc(__ballot_sync(0xffffffffu, at < hi && cu[at] <= least));
+        lo += n * step;
+        hi = min(hi, lo + step);
+    }
+    while (lo + 1 < batch && cu[lo + 1] <= t) ++lo;
+    return lo;
+}
+
+template <typename T, bool QUANT>
+__device__ __forceinline__ void store_row(const Row8<T>& row, const PagedTensor& to, const PagedTensor& scale,
+                                          bool store, int page, int h, int slot, int lane_of_row, int lanes_log2,
+                                          bool active) {
+    if constexpr (QUANT) {
+        float x[8];
+        row.get(x);
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float m = fabsf(x[i]);
+            if (m < INFINITY) top = fmaxf(top, m);  // false for NaN too
+        }
+        if (!active) top = 0.0f;
+        for (int off = 1 << lanes_log2 >> 1; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const int e = top > 0.0f ? scale_exponent(top) : 0;
+        const float inv = exp2_int(-e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], inv);  // exact, or below half of e4m3's least step
+        if (store) {
+            if (active) {
+                uint8_t* p = static_cast<uint8_t*>(to.p) + to.offset(page, h, slot) + lane_of_row * 8;
+                *reinterpret_cast<uint2*>(p) = to_e4m3(x);
+            }
+            if (lane_of_row == 0) static_cast<float*>(scale.p)[scale.offset(page, h, slot)] = exp2_int(e);
+        }
+    } else {
+        if (store && active) row.store(to.p, to.offset(page, h, slot) + lane_of_row * 8);
+    }
+}
+
+// A lane moves eight values of a token's keys and of its values in one head;
+// 2^lanes_log2 lanes share such a row (those behind head_dim idle), and a
+// thread takes ROWS rows, so that 2 * ROWS loads are under way while it finds
+// their pages.
+// Bound: HBM for prompts, the chain cu_seqlens -> length -> page for a step.
+template <typename T, bool QUANT, int ROWS>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
+    pdl_enter();
+    const int c = static_cast<int>(threadIdx.x) & ((1 << a.lanes_log2) - 1);
+    const uint32_t pass = kThreads >> a.lanes_log2;
+    const uint32_t row0 = blockIdx.x * (pass * ROWS) + (threadIdx.x >> a.lanes_log2);
+    const bool active = c * 8 < a.cache.head_dim;
+    Row8<T> k[ROWS], v[ROWS];
+    int t[ROWS], h[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        // rows behind the last repeat it and are not stored
+        const uint32_t row = min(row0 + i * pass, a.rows - 1);
+        t[i] = static_cast<int>(a.heads.div(row));
+        h[i] = static_cast<int>(row - t[i] * a.heads.d);
+        int64_t b = 0, s = t[i];
+        if (a.seqs.cu == nullptr) {
+            b = a.q_len.div(t[i]);
+            s -= b * a.q_len.d;
+        }
+        if (active) {
+            k[i].load(a.k, b * a.kb + s * a.ks + h[i] * a.kh + c * 8);
+            v[i].load(a.v, b * a.vb + s * a.vs + h[i] * a.vh + c * 8);
+        } else {
+            k[i].zero();
+            v[i].zero();
+        }
+    }
+    int b = a.seqs.cu == nullptr ? 0 : find_sequence(a.seqs.cu, a.seqs.batch, t[0]);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (a.seqs.cu == nullptr) {
+            b = static_cast<int>(a.q_len.div(t[i]));
+        } else {
+            while (b + 1 < a.seqs.batch && a.seqs.cu[b + 1] <= t[i]) ++b;
+        }
+        int first, n;
+        new_tokens(a.seqs, b, first, n);
+        const int at = t[i] - first;
+        const int pos = cached_tokens(a.seqs, b) - n + at;
+        bool store = row0 + i * pass < a.rows && at >= 0 && at < n && pos >= 0;
+        int slot = 0;
+        const int page = store ? page_of(a.seqs, a.cache, b, pos, slot) : -1;
+        store = page >= 0;
+        store_row<T, QUANT>(k[i], a.cache.k, a.cache.ks, store, page, h[i], slot, c, a.lanes_log2, active);
+        store_row<T, QUANT>(v[i], a.cache.v, a.cache.vs, store, page, h[i], slot, c, a.lanes_log2, active);
+    }
+}
+
+template <typename T>
+int launch_write(WriteArgs& a, bool quant, cudaStream_t st) {
+    a.lanes_log2 = lanes_log2(a.cache.head_dim, 8);
+    const int pass = kThreads >> a.lanes_log2;
+    const int each = rows_per_thread(a.rows, pass, 4, 4);
+    const dim3 grid(static_cast<unsigned>((int64_t{a.rows} + int64_t{pass} * each - 1) / (int64_t{pass} * each)));
+    const char* name = "kv_cache_write";
+    if (quant)
+        return each == 4 ? launch_ex(kv_write_kernel<T, true, 4>, grid, dim3(kThreads), 0, 1, st, a, name)
+                         : launch_ex(kv_write_kernel<T, true, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+    return each == 4 ? launch_ex(kv_write_kernel<T, false, 4>, grid, dim3(kThreads), 0, 1, st, a, name)
+                     : launch_ex(kv_write_kernel<T, false, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+}
+
+// -------------------------------------------------------------------- read
+struct ReadArgs {
+    void *k, *v;
+    int64_t kb, kh, ks, vb, vh, vs;
+    PagedCache cache;
+    PagedSeqs seqs;
+    FastDiv length, heads;
+    int64_t start;
+    uint32_t rows;  // batch * kv_heads * length
+    int lanes_log2;
+};
+
+// 16 e4m3 values (one 16-byte access).
+struct Row16Q {
+    uint4 w;
+
+    __device__ __forceinline__ void load(const void* base, int64_t at) {
+        w = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + at);
+    }
+    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+    template <typename T>
+    __device__ __forceinline__ void store(void* base, int64_t at, float scale) const {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = from_e4m3((u[half * 2 + i / 2] >> (16 * (i & 1))) & 0xffffu);
+                x[2 * i] = __fmul_rn(f.x, scale);
+                x[2 * i + 1] = __fmul_rn(f.y, scale);
+            }
+            Row8<T> r;
+            r.put(x);
+            r.store(base, at + half * 8);
+        }
+    }
+};
+
+// A lane moves 16 bytes of a row of the cache (a position's keys in one head)
+// and the same of its values, for ROWS rows. Rows run over positions first,
+// along a page and along the output.
+template <typename T, bool QUANT, int ROWS>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
+    pdl_enter();
+    using Held = std::conditional_t<QUANT, Row16Q, Row8<T>>;
+    constexpr int EACH = QUANT ? 16 : 8;
+    const int c = static_cast<int>(threadIdx.x) & ((1 << a.lanes_log2) - 1);
+    if (c * EACH >= a.cache.head_dim) return;
+    const uint32_t pass = kThreads >> a.lanes_log2;
+    const uint32_t row0 = blockIdx.x * (pass * ROWS) + (threadIdx.x >> a.lanes_log2);
+    Held k[ROWS], v[ROWS];
+    float ks[ROWS], vs[ROWS];
+    uint32_t j[ROWS];
+    int h[ROWS], b[ROWS], page[ROWS], slot[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const uint32_t row = min(row0 + i * pass, a.rows - 1);
+        const uint32_t bh = a.length.div(row);
+        j[i] = row - bh * a.length.d;
+        b[i] = static_cast<int>(a.heads.div(bh));
+        h[i] = static_cast<int>(bh - b[i] * a.heads.d);
+        const int64_t pos = a.start + j[i];
+        page[i] = -1;
+        slot[i] = 0;
+        if (pos < cached_tokens(a.seqs, b[i])) page[i] = page_of(a.seqs, a.cache, b[i], static_cast<int>(pos), slot[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        k[i].zero();
+        v[i].zero();
+        ks[i] = vs[i] = 0.0f;
+        if (page[i] >= 0) {
+            k[i].load(a.cache.k.p, a.cache.k.offset(page[i], h[i], slot[i]) + c * EACH);
+            v[i].load(a.cache.v.p, a.cache.v.offset(page[i], h[i], slot[i]) + c * EACH);
+            if constexpr (QUANT) {
+                ks[i] = static_cast<const float*>(a.cache.ks.p)[a.cache.ks.offset(page[i], h[i], slot[i])];
+                vs[i] = static_cast<const float*>(a.cache.vs.p)[a.cache.vs.offset(page[i], h[i], slot[i])];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (row0 + i * pass >= a.rows) return;
+        const int64_t ko = b[i] * a.kb + h[i] * a.kh + j[i] * a.ks + c * EACH;
+        const int64_t vo = b[i] * a.vb + h[i] * a.vh + j[i] * a.vs + c * EACH;
+        if constexpr (QUANT) {
+            k[i].template store<T>(a.k, ko, ks[i]);
+            v[i].template store<T>(a.v, vo, vs[i]);
+        } else {
+            k[i].store(a.k, ko);
+            v[i].store(a.v, vo);
+        }
+    }
+}
+
+template <typename T>
+int launch_read(ReadArgs& a, bool quant, cudaStream_t st) {
+    a.lanes_log2 = lanes_log2(a.cache.head_dim, quant ? 16 : 8);
+    const int pass = kThreads >> a.lanes_log2;
+    const int each = rows_per_thread(a.rows, pass, 2, 8);
+    const dim3 grid(static_cast<unsigned>((int64_t{a.rows} + int64_t{pass} * each - 1) / (int64_t{pass} * each)));
+    const char* name = "kv_cache_read";
+    if (quant)
+        return each == 2 ? launch_ex(kv_read_kernel<T, true, 2>, grid, dim3(kThreads), 0, 1, st, a, name)
+                         : launch_ex(kv_read_kernel<T, true, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+    return each == 2 ? launch_ex(kv_read_kernel<T, false, 2>, grid, dim3(kThreads), 0, 1, st, a, name)
+                     : launch_ex(kv_read_kernel<T, false, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+}
+
+// Pointer and the strides of axes longer than one are multiples of 16 bytes.
+bool rows16(const void* p, int64_t s0, int64_t n0, int64_t s1, int64_t n1, int64_t s2, int64_t n2, int es) {
+    return aligned16(p) && multiple16(s0, n0, es) && multiple16(s1, n1, es) && multiple16(s2, n2, es);
+}
+
+}  // namespace
+}  // namespace ako_b200
+
+using namespace ako_b200;
+
+extern "C" int ako_b200_kv_cache_write(const void* k, int64_t k_stride_b, int64_t k_stride_s, int64_t k_stride_h,
+                                       const void* v, int64_t v_stride_b, int64_t v_stride_s, int64_t v_stride_h,
+                                       const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,
+                                       int64_t tokens, int64_t q_len, int dtype, void* stream) {
+    clear_error();
+    const char* op = "ako_b200_kv_cache_write";
+    WriteArgs a{};
+    int es = 0;
+    int rc = make_cache(op, cache, dtype, a.cache, es);
+    if (rc) return rc;
+    if ((rc = make_seqs(op, batch, a.cache, tokens, q_len, a.seqs))) return rc;
+    if ((rc = refuse_if_wait_expired(op))) return rc;
+    if (tokens == 0 || a.seqs.batch == 0 || a.seqs.max_kv == 0) return AKO_B200_OK;
+    if (tokens * a.cache.kv_heads > INT_MAX)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: tokens * kv_heads must be < 2^31", op);
+    if (k == nullptr || v == nullptr)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k or v is a null pointer", op);
+    const bool uniform = a.seqs.cu == nullptr;
+    const int64_t nb = uniform ? a.seqs.batch : 1, ns = uniform ? q_len : tokens;
+    const int in = dtype_size(dtype);
+    if (!rows16(k, k_stride_b, nb, k_stride_s, ns, k_stride_h, a.cache.kv_heads, in) ||
+        !rows16(v, v_stride_b, nb, v_stride_s, ns, v_stride_h, a.cache.kv_heads, in))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k, v and their strides must be multiples of 16 bytes", op);
+    a.k = k;
+    a.v = v;
+    a.kb = k_stride_b;
+    a.ks = k_stride_s;
+    a.kh = k_stride_h;
+    a.vb = v_stride_b;
+    a.vs = v_stride_s;
+    a.vh = v_stride_h;
+    a.heads = FastDiv::make(static_cast<uint32_t>(a.cache.kv_heads));
+    a.q_len = FastDiv::make(static_cast<uint32_t>(uniform ? q_len : 1));
+    a.rows = static_cast<uint32_t>(tokens * a.cache.kv_heads);
+    const bool quant = cache->dtype == AKO_B200_E4M3;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case AKO_B200_F32: return launch_write<float>(a, quant, st);
+        case AKO_B200_F16: return launch_write<__half>(a, quant, st);
+        default: return launch_write<__nv_bfloat16>(a, quant, st);
+    }
+}
+
+extern "C" int ako_b200_kv_cache_read(const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,
+                                      int64_t start, int64_t length, void* k_out, int64_t k_stride_b,
+                                      int64_t k_stride_h, int64_t k_stride_s, void* v_out, int64_t v_stride_b,
+                                      int64_t v_stride_h, int64_t v_stride_s, int dtype, void* stream) {
+    clear_error();
+    const char* op = "ako_b200_kv_cache_read";
+    ReadArgs a{};
+    int es = 0;
+    int rc = make_cache(op, cache, dtype, a.cache, es);
+    if (rc) return rc;
+    // the new tokens' rows play no part in a read
+    if ((rc = make_seqs(op, batch, a.cache, 0, 0, a.seqs))) return rc;
+    if ((rc = refuse_if_wait_expired(op))) return rc;
+    if (start < 0 || length < 0 || start > INT_MAX || length > INT_MAX)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: start and length must be within 0 .. 2^31 - 1", op);
+    if (length == 0 || a.seqs.batch == 0) return AKO_B200_OK;
+    if (int64_t{a.seqs.batch} * a.cache.kv_heads > INT_MAX / length)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: batch * kv_heads * length must be < 2^31", op);
+    if (k_out == nullptr || v_out == nullptr)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k_out or v_out is a null pointer", op);
+    const int out = dtype_size(dtype);
+    if (!rows16(k_out, k_stride_b, a.seqs.batch, k_stride_h, a.cache.kv_heads, k_stride_s, length, out) ||
+        !rows16(v_out, v_stride_b, a.seqs.batch, v_stride_h, a.cache.kv_heads, v_stride_s, length, out))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT,
+                         "%s: k_out, v_out and their strides must be multiples of 16 bytes", op);
+    a.k = k_out;
+    a.v = v_out;
+    a.kb = k_stride_b;
+    a.kh = k_stride_h;
+    a.ks = k_stride_s;
+    a.vb = v_stride_b;
+    a.vh = v_stride_h;
+    a.vs = v_stride_s;
+    a.length = FastDiv::make(static_cast<uint32_t>(length));
+    a.heads = FastDiv::make(static_cast<uint32_t>(a.cache.kv_heads));
+    a.start = start;
+    a.rows = static_cast<uint32_t>(int64_t{a.seqs.batch} * a.cache.kv_heads * length);
+    const bool quant = cache->dtype == AKO_B200_E4M3;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case AKO_B200_F32: return launch_read<float>(a, quant, st);
+        case AKO_B200_F16: return launch_read<__half>(a, quant, st);
+        default: return launch_read<__nv_bfloat16>(a, quant, st);
+    }
+}

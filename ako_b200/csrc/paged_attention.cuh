@@ -1,0 +1,293 @@
+// Attention over a paged cache: its arguments, the division of the work, and
+// what its kernels share.
+#pragma once
+
+#include "paged.cuh"
+
+namespace ako_b200 {
+
+struct AttnArgs {
+    const void* q;
+    void* out;
+    int64_t qb, qs, qh, ob, os, oh;
+    PagedCache cache;
+    PagedSeqs seqs;
+    int group;       // q heads that share a kv head
+    int window;      // 0: none
+    int sinks;
+    float scale;     // scale * log2(e)
+    FastDiv by_group;
+    float* partial;  // (2 * ctas) blocks of PartialBlock
+    int4* joins;     // per CTA: the item that it begins and others end
+};
+
+// ------------------------------------------------------------------- work
+// The rows that one kv head of one sequence answers are its new tokens times
+// the q heads that share it, token by token: row r is token r / group, head
+// r % group of the group. A tile of TILE rows against one kv head is an item;
+// its keys come in tiles of BN. All items' key tiles, in the order (sequence,
+// row tile, kv head, key tile), form one list, and CTA c of N takes the part
+// from c * total / N up to (c + 1) * total / N of it. So every CTA gets the
+// same number of key tiles whatever the sequences' lengths are, and no CTA
+// holds parts of more than one item that it does not own whole at each end.
+struct Item {
+    int b, rt, h;           // sequence, row tile, kv head
+    int first, n, kv;       // the sequence's first new token, new and cached tokens
+    int row0, rows;         // rows of this item: row0 .. row0 + rows - 1
+    int p_lo, p_hi;         // positions of its first and last row
+    int win_lo;             // no row sees a key below it that is not a sink
+    int sink_tiles, tile_lo, tiles;  // key tiles: [0, sink_tiles) and then from tile_lo on
+};
+
+template <int TILE, int BN>
+__device__ __forceinline__ void item_geometry(const AttnArgs& a, Item& it) {
+    it.row0 = it.rt * TILE;
+    it.rows = min(TILE, it.n * a.group - it.row0);
+    const int before = it.kv - it.n;
+    it.p_lo = before + static_cast<int>(a.by_group.div(it.row0));
+    it.p_hi = before + static_cast<int>(a.by_group.div(it.row0 + it.rows - 1));
+    const int end = max(it.p_hi + 1, 0);
+    it.win_lo = a.window > 0 ? max(it.p_lo - a.window + 1, 0) : 0;
+    it.tile_lo = it.win_lo / BN;
+    it.sink_tiles = min((min(a.sinks, end) + BN - 1) / BN, it.tile_lo);
+    // an item without a key still has its rows to write: one tile, all masked
+    it.tiles = max(it.sink_tiles + (end + BN - 1) / BN - it.tile_lo, 1);
+}
+
+__device__ __forceinline__ int key_tile(const Item& it, int t) {
+    return t < it.sink_tiles ? t : it.tile_lo + (t - it.sink_tiles);
+}
+
+template <int TILE>
+__device__ __forceinline__ int row_tiles(const AttnArgs& a, int n) { return (n * a.group + TILE - 1) / TILE; }
+
+// Key tiles of sequence `b` over its row tiles and heads. All lanes of a warp
+// call it, with b = -1 for none: sequences with many row tiles are summed by
+// the whole warp.
+template <int TILE, int BN>
+__device__ __forceinline__ int64_t sequence_tiles(const AttnArgs& a, int b) {
+    Item it;
+    it.n = 0;
+    it.kv = 0;
+    if (b >= 0) {
+        new_tokens(a.seqs, b, it.first, it.n);
+        it.kv = cached_tokens(a.seqs, b);
+    }
+    const int nrt = row_tiles<TILE>(a, it.n);
+    int64_t sum = 0;
+    if (nrt <= 4) {
+        for (it.rt = 0; it.rt < nrt; ++it.rt) {
+            item_geometry<TILE, BN>(a, it);
+            sum += it.tiles;
+        }
+    }
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    for (unsigned many = __ballot_sync(0xffffffffu, nrt > 4); many != 0; many &= many - 1) {
+        const int src = __ffs(many) - 1;
+        Item o;
+        o.n = __shfl_sync(0xffffffffu, it.n, src);
+        o.kv = __shfl_sync(0xffffffffu, it.kv, src);
+        const int tiles = __shfl_sync(0xffffffffu, nrt, src);
+        int64_t s = 0;
+        for (o.rt = lane; o.rt < tiles; o.rt += 32) {
+            item_geometry<TILE, BN>(a, o);
+            s += o.tiles;
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        if (lane == src) sum = s;
+    }
+    return sum * a.cache.kv_heads;
+}
+
+// This CTA's part of the list, and the item and key tile where it begins.
+struct Share {
+    int64_t begin, end, total;
+    int ctas;  // CTAs that take part
+    Item it;
+    int t;  // key tile within the item
+};
+
+struct ShareScratch {
+    int64_t warp_sum[32];
+    int64_t at;  // begin, counted from the sequence's first tile
+    int b;
+};
+
+// All threads of the CTA call it (THREADS a multiple of 32). False when this
+// CTA has nothing to do.
+template <int TILE, int BN, int THREADS>
+__device__ bool find_share(const AttnArgs& a, int per_cta, ShareScratch& sm, Share& out) {
+    constexpr int WARPS = THREADS / 32;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+    const int chunks = (a.seqs.batch + THREADS - 1) / THREADS;
+    int64_t mine = 0, total = 0;
+    for (int i = 0; i < chunks; ++i) {
+        const int b = i * THREADS + tid;
+        mine = sequence_tiles<TILE, BN>(a, b < a.seqs.batch ? b : -1);
+        total += mine;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (lane == 0) sm.warp_sum[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) total += sm.warp_sum[i];
+    __syncthreads();
+    const int64_t most = (total + per_cta - 1) / per_cta;
+    out.ctas = static_cast<int>(most < gridDim.x ? most : gridDim.x);
+    if (static_cast<int>(blockIdx.x) >= out.ctas) return false;
+    out.total = total;
+    out.begin = blockIdx.x * total / out.ctas;
+    out.end = (blockIdx.x + 1) * total / out.ctas;
+    int64_t before = 0;
+    for (int i = 0; i < chunks; ++i) {
+        const int b = i * THREADS + tid;
+        if (chunks > 1) mine = sequence_tiles<TILE, BN>(a, b < a.seqs.batch ? b : -1);
+        int64_t incl = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += o;
+        }
+        if (lane == 31) sm.warp_sum[warp] = incl;
+        __syncthreads();
+        int64_t base = before;
+        for (int w = 0; w < WARPS; ++w) {
+            if (w == warp) incl += base;
+            base += sm.warp_sum[w];
+        }
+        before = base;
+        if (out.begin >= incl - mine && out.begin < incl) {
+            sm.b = b;
+            sm.at = out.begin - (incl - mine);
+        }
+        __syncthreads();
+        if (before > out.begin) break;
+    }
+    Item& it = out.it;
+    it.b = sm.b;
+    int64_t at = sm.at;
+    new_tokens(a.seqs, it.b, it.first, it.n);
+    it.kv = cached_tokens(a.seqs, it.b);
+    const int last = row_tiles<TILE>(a, it.n) - 1;
+    for (it.rt = 0;; ++it.rt) {
+        item_geometry<TILE, BN>(a, it);
+        const int64_t all = static_cast<int64_t>(it.tiles) * a.cache.kv_heads;
+        if (at < all || it.rt >= last) break;
+        at -= all;
+    }
+    it.h = static_cast<int>(at / it.tiles);
+    out.t = static_cast<int>(at - static_cast<int64_t>(it.h) * it.tiles);
+    return true;
+}
+
+// The item behind `it` in the list; false behind the last.
+template <int TILE, int BN>
+__device__ __forceinline__ bool next_item(const AttnArgs& a, Item& it) {
+    if (++it.h < a.cache.kv_heads) return true;
+    it.h = 0;
+    if (++it.rt < row_tiles<TILE>(a, it.n)) {
+        item_geometry<TILE, BN>(a, it);
+        return true;
+    }
+    it.rt = 0;
+    while (++it.b < a.seqs.batch) {
+        new_tokens(a.seqs, it.b, it.first, it.n);
+        if (it.n > 0) {
+            it.kv = cached_tokens(a.seqs, it.b);
+            item_geometry<TILE, BN>(a, it);
+            return true;
+        }
+    }
+    return false;
+}
+
+// The CTA that tile `t` of the list belongs to.
+__device__ __forceinline__ int owner(const Share& s, int64_t t) {
+    return static_cast<int>(((t + 1) * s.ctas - 1) / s.total);
+}
+
+// ---------------------------------------------------------------- partials
+// A CTA writes at most two partial results: block 2c, of an item that an
+// earlier CTA begins, and block 2c + 1, of an item that it begins and a later
+// one ends. Each holds the rows' maxima (log2 domain), sums, and sums of
+// weighted values. CTA c's entry of `joins` says who else has parts of the
+// second: {b, rt, h, last CTA}, or {-1, ...}.
+template <int ROWS, int DPAD>
+struct PartialBlock {
+    float m[ROWS], l[ROWS];
+    float o[ROWS][DPAD];
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Element offset of row r of an item in q (or out) with strides b, s, h.
+__device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Item& it, int r, int64_t sb, int64_t ss,
+                                              int64_t sh) {
+    const int i = static_cast<int>(a.by_group.div(r));
+    const int64_t head = static_cast<int64_t>(it.h) * a.group + (r - i * a.group);
+    if (a.seqs.cu == nullptr) return it.b * sb + i * ss + head * sh;
+    return static_cast<int64_t>(it.first + i) * ss + head * sh;
+}
+
+// Four columns of an item's row: weighted sum over sum of weights, rounded
+// once; zero where no key was seen.
+template <typename T>
+__device__ __forceinline__ void write_row(const AttnArgs& a, const Item& it, int r, int c, const float4& acc, float sum) {
+    if (c >= a.cache.head_dim) return;
+    const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
+    Packed<T, 4> y;
+    put2(y, 0, acc.x * inv, acc.y * inv);
+    put2(y, 2, acc.z * inv, acc.w * inv);
+    *reinterpret_cast<Packed<T, 4>*>(static_cast<T*>(a.out) + row_offset(a, it, it.row0 + r, a.ob, a.os, a.oh) + c) = y;
+}
+
+// Joins the parts of the items that several CTAs took: CTA (c, y) the rows
+// [y * 4 WARPS...) of the item that CTA c of the grid before it began.
+template <typename T, int ROWS, int DPAD>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
+    pdl_enter();
+    const int4 j = a.joins[blockIdx.x];
+    if (j.x < 0) return;
+    using Block = PartialBlock<ROWS, DPAD>;
+    constexpr int LANES = DPAD / 4, STEP = 128 / LANES;
+    Item it;
+    it.b = j.x;
+    it.rt = j.y;
+    it.h = j.z;
+    new_tokens(a.seqs, it.b, it.first, it.n);
+    it.row0 = it.rt * ROWS;
+    it.rows = min(ROWS, it.n * a.group - it.row0);
+    const int r = static_cast<int>(blockIdx.y) * STEP + static_cast<int>(threadIdx.x) / LANES;
+    const int c = static_cast<int>(threadIdx.x) % LANES * 4;
+    if (r >= it.rows) return;
+    const Block* const first = reinterpret_cast<const Block*>(a.partial) + 2 * blockIdx.x + 1;
+    const Block* const others = reinterpret_cast<const Block*>(a.partial) + 2 * (blockIdx.x + 1);
+    const int n = j.w - static_cast<int>(blockIdx.x);  // CTAs behind the first
+    float top = first->m[r];
+    for (int i = 0; i < n; ++i) top = fmaxf(top, others[2 * i].m[r]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float f = ex2(first->m[r] - ref), sum = f * first->l[r];
+    float4 v = *reinterpret_cast<const float4*>(&first->o[r][c]);
+    float4 acc = make_float4(f * v.x, f * v.y, f * v.z, f * v.w);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const Block& b = others[2 * i];
+        f = ex2(b.m[r] - ref);
+        v = *reinterpret_cast<const float4*>(&b.o[r][c]);
+        sum = fmaf(f, b.l[r], sum);
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+    }
+    write_row<T>(a, it, r, c, acc, sum);
+}
+
+}  // namespace ako_b200

@@ -1,0 +1,560 @@
+// Attention of few rows per sequence and kv head over a paged cache: the
+// decoding step, and the general form of the operator.
+//
+// Each warp takes 16 keys at a time through its own ring of asynchronous
+// copies and keeps a running maximum, sum and weighted sum of values; a CTA's
+// four warps take neighbouring 16 keys of each 64-key tile and join their
+// sums once per item, so nothing in the loop waits for another warp.
+//
+// The products are taken transposed, keys along M: S^T = K Q^T and
+// O^T = V^T P^T with m16n8k16, so that the rows, of which there are few, fill
+// an N of 8 and not an M of 16. S^T's accumulators become P^T's operand by one
+// 8x8 transpose in registers (movmatrix).
+//
+// Bound: HBM, by the keys and values read once.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "paged_attention.cuh"
+
+namespace ako_b200 {
+
+constexpr int kRowsWarps = 4;
+constexpr int kRowsThreads = kRowsWarps * 32;
+constexpr int kWarpKeys = 16;
+constexpr int kRowsKeys = kRowsWarps * kWarpKeys;  // keys of a tile
+
+// 16-byte asynchronous copy; zeros instead when `real` is false.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(real ? 16 : 0)
+                 : "memory");
+}
+
+__device__ __forceinline__ void cp_async4_or_zero(uint32_t smem, const void* gmem, bool real) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem), "l"(gmem), "r"(real ? 4 : 0) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// d += a b, m16n8k16, fp32 sums.
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    Packed<T, 2> p;
+    put2(p, 0, lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// Two e4m3 values, the low 16 bits of `pair`, as two fp16 (exact).
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t pair) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(pair));
+    return r;
+}
+
+template <typename T>
+struct Half16;  // bit patterns of a 16-bit type
+template <>
+struct Half16<__half> {
+    static constexpr uint32_t inf = 0x7c00, one = 0x3c00;
+};
+template <>
+struct Half16<__nv_bfloat16> {
+    static constexpr uint32_t inf = 0x7f80, one = 0x3f80;
+};
+
+// Shape of an instantiation: T the activations' type, QUANT an e4m3 cache,
+// DPAD the head's width rounded up, NT tiles of 8 rows.
+template <typename T, bool QUANT, int DPAD, int NT>
+struct RowsShape {
+    // An e4m3 cache is multiplied in fp16, which holds its values exactly; q
+    // is scaled by a power of two per row to fit.
+    using M = std::conditional_t<QUANT, __half, T>;
+    static constexpr int kRows = NT * 8;
+    static constexpr int kRowBytes = DPAD * (QUANT ? 1 : 2);
+    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kStageBytes = 2 * kWarpKeys * kRowBytes + (QUANT ? 2 * kWarpKeys * 4 : 0) + 16;
+    // Bytes under way per SM are what the rate follows from: 2 CTAs of four
+    // 24 KB rings (16-bit, head 128).
+    static constexpr int kStages = QUANT ? 4 : 3;
+    static constexpr int kRing = kRowsWarps * kStages * kStageBytes;
+    static constexpr int kJoinStride = DPAD + 4;  // floats; keeps the four column groups on different banks
+    static constexpr int kJoin = kRowsWarps * kRows * (kJoinStride + 2) * 4;
+    static constexpr int kQStride = DPAD + 8;
+    static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kRows * (kQStride * 2 + 8);
+    static constexpr int kFit = 227 * 1024 / (kSmem + 2048);
+    static constexpr int kMost = NT >= 4 ? 2 : NT == 2 ? 3 : 4;
+    static constexpr int kCtas = kFit < kMost ? kFit : kMost;  // per SM
+};
+
+// Chunk c of a key's row in shared memory, so that eight rows' chunks that are
+// read together lie in different banks. K of a quantised cache is read as two
+// rows of four chunks at a time, everything else as eight rows of one.
+template <bool QUANT, int DPAD, bool KEYS>
+__device__ __forceinline__ int swizzled(int row, int c) {
+    if constexpr (!QUANT) return c ^ (row & 7);
+    if constexpr (KEYS) return DPAD == 128 ? c ^ ((row & 1) << 2) : c;
+    return DPAD == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3);
+}
+
+template <typename T, bool QUANT, int DPAD, int NT>
+__global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::kCtas))
+    attn_rows_kernel(const AttnArgs a) {
+    pdl_enter();
+    using Shape = RowsShape<T, QUANT, DPAD, NT>;
+    using M = typename Shape::M;
+    using Block = PartialBlock<Shape::kRows, DPAD>;
+    constexpr int ROWS = Shape::kRows, KS = DPAD / 16, STAGES = Shape::kStages, CHUNKS = Shape::kChunks;
+    constexpr int ROWB = Shape::kRowBytes;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ ShareScratch scratch;
+    M* const sq = reinterpret_cast<M*>(smem + Shape::kSmem - ROWS * (Shape::kQStride * 2 + 8));
+    float* const row_factor = reinterpret_cast<float*>(sq + ROWS * Shape::kQStride);
+    int* const row_pos = reinterpret_cast<int*>(row_factor + ROWS);
+
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t4 = lane & 3;  // row and column pair of a fragment
+    const int dim = a.cache.head_dim;
+
+    if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    Share share;
+    if (!find_share<ROWS, kRowsKeys, kRowsThreads>(a, 1, scratch, share)) return;
+    Item& it = share.it;
+
+    uint8_t* const ring = smem + warp * (STAGES * Shape::kStageBytes);
+    const uint32_t ring_addr = smem_addr(ring);
+
+    int64_t at = share.begin;
+    while (true) {
+        const int t_end = static_cast<int>(min(static_cast<int64_t>(it.tiles), share.t + (share.end - at)));
+
+        // ------------------------------------------------ keys under way
+        // Lanes 0-15 look after the 16 keys' rows of K, lanes 16-31 of V.
+        const PagedTensor& mine = lane < 16 ? a.cache.k : a.cache.v;
+        int next_page = -1, next_slot = 0;
+        auto look_up = [&](int t) {
+            const int key = key_tile(it, t) * kRowsKeys + warp * kWarpKeys + (lane & 15);
+            next_page = -1;
+            if (t < t_end && key <= it.p_hi && (key >= it.win_lo || key < a.sinks))
+                next_page = page_of(a.seqs, a.cache, it.b, key, next_slot);
+        };
+        auto issue = [&](int t, int stage) {
+            if (t < t_end) {
+                const int page = next_page, slot = next_slot;
+                look_up(t + 1);
+                const int64_t off = page >= 0 ? mine.offset(page, it.h, slot) : -1;
+                const uint32_t to = ring_addr + stage * Shape::kStageBytes;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const uint8_t* base = static_cast<const uint8_t*>(kv == 0 ? a.cache.k.p : a.cache.v.p);
+#pragma unroll
+                    for (int i = 0; i < kWarpKeys * CHUNKS / 32; ++i) {
+                        const int row = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
+                        const int64_t o = __shfl_sync(0xffffffffu, off, kv * 16 + row);
+                        const bool real = o >= 0 && c * 16 < dim * (QUANT ? 1 : 2);
+                        const int sc = kv == 0 ? swizzled<QUANT, DPAD, true>(row, c) : swizzled<QUANT, DPAD, false>(row, c);
+                        cp_async16_or_zero(to + (kv * kWarpKeys + row) * ROWB + sc * 16,
+                                           real ? base + o * (QUANT ? 1 : 2) + c * 16 : base, real);
+                    }
+                }
+                if constexpr (QUANT) {
+                    const PagedTensor& st = lane < 16 ? a.cache.ks : a.cache.vs;
+                    const float* p = static_cast<const float*>(st.p);
+                    cp_async4_or_zero(to + 2 * kWarpKeys * ROWB + lane * 4,
+                                      page >= 0 ? p + st.offset(page, it.h, slot) : p, page >= 0);
+                }
+                const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+                if (lane == 0)
+                    *reinterpret_cast<volatile uint32_t*>(ring + (stage + 1) * Shape::kStageBytes - 16) = there & 0xffffu;
+            }
+            cp_async_commit();
+        };
+        look_up(share.t);
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) issue(share.t + i, i);
+
+        // ------------------------------------------------------------ rows
+        for (int r = warp; r < ROWS; r += kRowsWarps) {
+            constexpr int EACH = DPAD / 32;  // 4 or 2 elements per lane
+            float x[EACH] = {};
+            if (r < it.rows && lane * EACH < dim) {
+                const T* p = static_cast<const T*>(a.q) + row_offset(a, it, it.row0 + r, a.qb, a.qs, a.qh) + lane * EACH;
+                const Packed<T, EACH> v = *reinterpret_cast<const Packed<T, EACH>*>(p);
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) x[i] = to_f32(v.v[i]);
+            }
+            float factor = 1.0f;
+            if constexpr (QUANT && !std::is_same_v<T, __half>) {
+                // power of two that takes the row's largest value into [2^8, 2^9): what fp16 then
+                // flushes is 2^-33 of it
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                if (top > 0.0f && top < INFINITY) {
+                    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 8, -126), 118);
+                    const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+                    for (int i = 0; i < EACH; ++i) x[i] = __fmul_rn(x[i], inv);
+                    factor = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                }
+            }
+            Packed<M, EACH> w;
+#pragma unroll
+            for (int i = 0; i < EACH; i += 2) put2(w, i, x[i], x[i + 1]);
+            *reinterpret_cast<Packed<M, EACH>*>(sq + r * Shape::kQStride + lane * EACH) = w;
+            if (lane == 0) {
+                row_factor[r] = factor;
+                row_pos[r] = r < it.rows ? it.kv - it.n + static_cast<int>(a.by_group.div(it.row0 + r)) : it.p_hi;
+            }
+        }
+        __syncthreads();
+
+        // B operand of S^T: q's rows along N. With an e4m3 cache a k-step
+        // takes its head columns in the order that K's 16-byte reads give.
+        auto q_fragment = [&](int ks, int nt, uint32_t& b0, uint32_t& b1) {
+            const M* p = sq + (nt * 8 + g) * Shape::kQStride;
+            if constexpr (QUANT) {
+                p += (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4;
+                b0 = *reinterpret_cast<const uint32_t*>(p);
+                b1 = *reinterpret_cast<const uint32_t*>(p + 2);
+            } else {
+                p += ks * 16 + t4 * 2;
+                b0 = *reinterpret_cast<const uint32_t*>(p);
+                b1 = *reinterpret_cast<const uint32_t*>(p + 8);
+            }
+        };
+        constexpr bool HOLD = NT <= 2;  // q's fragments stay in registers
+        uint32_t qf[HOLD ? KS : 1][HOLD ? NT : 1][2];
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) q_fragment(ks, nt, qf[ks][nt][0], qf[ks][nt][1]);
+        }
+        float m[NT][2], l[NT][2], factor[NT][2];
+        int pos[NT][2];
+        float o[KS][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[nt][e] = -INFINITY;
+                l[nt][e] = 0.0f;
+                factor[nt][e] = QUANT ? row_factor[nt * 8 + t4 * 2 + e] : 1.0f;
+                pos[nt][e] = row_pos[nt * 8 + t4 * 2 + e];
+            }
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.0f;
+        }
+
+        // ------------------------------------------------------------ keys
+        int stage = 0;
+        for (int t = share.t; t < t_end; ++t) {
+            const int to = stage == 0 ? STAGES - 1 : stage - 1;
+            issue(t + STAGES - 1, to);
+            cp_async_wait<STAGES - 1>();
+            __syncwarp();
+            const uint8_t* const st = ring + stage * Shape::kStageBytes;
+            const uint32_t k_addr = ring_addr + stage * Shape::kStageBytes, v_addr = k_addr + kWarpKeys * ROWB;
+            const uint32_t there = *reinterpret_cast<const volatile uint32_t*>(st + Shape::kStageBytes - 16);
+            const int key0 = key_tile(it, t) * kRowsKeys + warp * kWarpKeys;
+
+            float x[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[nt][e] = 0.0f;
+            auto scores = [&](int ks, const uint32_t(&kf)[4]) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if constexpr (HOLD) {
+                        mma16816<M>(x[nt], kf, qf[ks][nt][0], qf[ks][nt][1]);
+                    } else {
+                        uint32_t b0, b1;
+                        q_fragment(ks, nt, b0, b1);
+                        mma16816<M>(x[nt], kf, b0, b1);
+                    }
+                }
+            };
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int j = 0; j < DPAD / 64; ++j) {
+                    const uint4 lo = *reinterpret_cast<const uint4*>(
+                        st + g * ROWB + swizzled<QUANT, DPAD, true>(g, j * 4 + t4) * 16);
+                    const uint4 hi = *reinterpret_cast<const uint4*>(
+                        st + (g + 8) * ROWB + swizzled<QUANT, DPAD, true>(g + 8, j * 4 + t4) * 16);
+                    const uint32_t u[4] = {lo.x, lo.y, lo.z, lo.w}, w[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t kf[4] = {e4m3x2_to_half2(u[i]), e4m3x2_to_half2(w[i]),
+                                                e4m3x2_to_half2(u[i] >> 16), e4m3x2_to_half2(w[i] >> 16)};
+                        scores(j * 4 + i, kf);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    uint32_t kf[4];
+                    const int row = lane & 15;
+                    ldmatrix4(kf, k_addr + row * ROWB + swizzled<QUANT, DPAD, true>(row, 2 * ks + (lane >> 4)) * 16);
+                    scores(ks, kf);
+                }
+            }
+
+            // Scores in units of log2(e). A quantised value's scale joins its key's
+            // score as a logarithm, so that the weights of the second product,
+            // exp2(x - max) of the joint score, fit in 16 bits whatever the scales
+            // are; the sum of weights takes it out again. A scale of zero counts as
+            // 2^-100 there.
+            float kc[2] = {a.scale, a.scale}, lv[2] = {0.0f, 0.0f}, unscale[2] = {1.0f, 1.0f};
+            if constexpr (QUANT) {
+                const float* sc = reinterpret_cast<const float*>(st + 2 * kWarpKeys * ROWB);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    kc[e] = a.scale * sc[g + 8 * e];
+                    const float v = fmaxf(sc[16 + g + 8 * e], 0x1p-100f);
+                    lv[e] = __log2f(v);
+                    unscale[e] = __fdividef(1.0f, v);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (QUANT) x[nt][e] = fmaf(x[nt][e] * factor[nt][e & 1], kc[e >> 1], lv[e >> 1]);
+                    else x[nt][e] *= a.scale;
+                }
+            const bool whole = there == 0xffffu && key0 + kWarpKeys - 1 <= it.p_lo &&
+                               (a.window == 0 || key0 > it.p_hi - a.window || key0 + kWarpKeys <= a.sinks);
+            unsigned seen = 0xffffffffu;
+            if (!whole) {
+                seen = 0;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = g + 8 * (e >> 1), key = key0 + i, p = pos[nt][e & 1];
+                        const bool sees = (there >> i & 1) != 0 && key <= p &&
+                                          (a.window == 0 || key > p - a.window || key < a.sinks);
+                        if (sees) seen |= 1u << (nt * 4 + e);
+                        else x[nt][e] = -INFINITY;
+                    }
+            }
+            bool grew = false;
+            float alpha[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(x[nt][e], x[nt][e + 2]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float mn = fmaxf(m[nt][e], top);
+                    const float ref = mn == -INFINITY ? 0.0f : mn;
+                    alpha[nt][e] = ex2(m[nt][e] - ref);
+                    grew |= mn != m[nt][e];
+                    m[nt][e] = mn;
+                    x[nt][e] = ex2(x[nt][e] - ref);
+                    x[nt][e + 2] = ex2(x[nt][e + 2] - ref);
+                    l[nt][e] = fmaf(l[nt][e], alpha[nt][e],
+                                    QUANT ? fmaf(x[nt][e], unscale[0], x[nt][e + 2] * unscale[1]) : x[nt][e] + x[nt][e + 2]);
+                }
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[mt][nt][e] *= alpha[nt][e & 1];
+            }
+            // The weights go to the 16-bit operand type, as the values are; the sum above took them in fp32.
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                pf[nt][0] = transpose8x8(pack2<M>(x[nt][0], x[nt][1]));
+                pf[nt][1] = transpose8x8(pack2<M>(x[nt][2], x[nt][3]));
+            }
+            auto values = [&](int mt, uint32_t(&vf)[4]) {
+                if (!whole) {
+                    // A weight of zero does not keep an infinity or NaN out of a product, so a
+                    // value that is not finite is taken out of the operand and, for the rows that
+                    // see it, counted by a product of its own.
+                    using B = Half16<M>;
+                    uint32_t bad[4], any = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        bad[i] = __vcmpgeu2(vf[i] & 0x7fff7fffu, B::inf | B::inf << 16);
+                        any |= bad[i];
+                    }
+                    if (__any_sync(0xffffffffu, any != 0)) {
+                        constexpr uint32_t ONE = B::one | B::one << 16;
+                        uint32_t kind[3][4];  // +inf, -inf, NaN as ones
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            kind[0][i] = __vcmpeq2(vf[i], B::inf | B::inf << 16) & ONE;
+                            kind[1][i] = __vcmpeq2(vf[i], (B::inf | B::inf << 16) | 0x80008000u) & ONE;
+                            kind[2][i] = __vcmpgtu2(vf[i] & 0x7fff7fffu, B::inf | B::inf << 16) & ONE;
+                            vf[i] &= ~bad[i];
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            auto one = [&](int e) { return seen >> (nt * 4 + e) & 1 ? 1.0f : 0.0f; };
+                            const uint32_t b0 = transpose8x8(pack2<M>(one(0), one(1)));
+                            const uint32_t b1 = transpose8x8(pack2<M>(one(2), one(3)));
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) {
+                                float n[4] = {};
+                                mma16816<M>(n, kind[k], b0, b1);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (n[e] > 0.0f) o[mt][nt][e] += k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<M>(o[mt][nt], vf, pf[nt][0], pf[nt][1]);
+            };
+            if constexpr (QUANT) {
+                // A 16-bit element of V is the pair (2u, 2u + 1) of a tile's 16 head columns:
+                // its transposed matrices give rows 2u and 2u + 1, which are taken as rows
+                // u and u + 8 of the operand.
+#pragma unroll
+                for (int mt = 0; mt < KS; mt += 2) {
+                    uint32_t r[4];
+                    const int row = (lane & 7) + 8 * ((lane >> 3) & 1);
+                    ldmatrix4_trans(r, v_addr + row * ROWB + swizzled<QUANT, DPAD, false>(row, mt + (lane >> 4)) * 16);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t vf[4];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            vf[2 * j] = e4m3x2_to_half2(__byte_perm(r[2 * i + j], 0, 0x4420));
+                            vf[2 * j + 1] = e4m3x2_to_half2(__byte_perm(r[2 * i + j], 0, 0x4431));
+                        }
+                        values(mt + i, vf);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) {
+                    uint32_t vf[4];
+                    const int row = (lane & 7) + 8 * (lane >> 4);
+                    ldmatrix4_trans(vf, v_addr + row * ROWB +
+                                            swizzled<QUANT, DPAD, false>(row, 2 * mt + ((lane >> 3) & 1)) * 16);
+                    values(mt, vf);
+                }
+            }
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            __syncwarp();  // the stage is read before the next copies into it
+        }
+
+        // ------------------------------------------------------------ join
+        __syncthreads();  // the rings become the warps' results
+        float* const join_o = reinterpret_cast<float*>(smem);
+        float* const join_m = join_o + kRowsWarps * ROWS * Shape::kJoinStride;
+        float* const join_l = join_m + kRowsWarps * ROWS;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float s = l[nt][e];
+                s += __shfl_xor_sync(0xffffffffu, s, 4);
+                s += __shfl_xor_sync(0xffffffffu, s, 8);
+                s += __shfl_xor_sync(0xffffffffu, s, 16);
+                const int r = nt * 8 + t4 * 2 + e;
+                if (g == 0) {
+                    join_m[warp * ROWS + r] = m[nt][e];
+                    join_l[warp * ROWS + r] = s;
+                }
+                float* const to = join_o + (warp * ROWS + r) * Shape::kJoinStride;
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) {
+                    to[mt * 16 + (QUANT ? 2 * g : g)] = o[mt][nt][e];
+                    to[mt * 16 + (QUANT ? 2 * g + 1 : g + 8)] = o[mt][nt][e + 2];
+                }
+            }
+        __syncthreads();
+        const bool begins = share.t == 0, ends = t_end == it.tiles;
+        Block* const block = reinterpret_cast<Block*>(a.partial) + 2 * blockIdx.x + (begins ? 1 : 0);
+        constexpr int LANES = DPAD / 4;  // of a row
+        for (int r = tid / LANES; r < it.rows; r += kRowsThreads / LANES) {
+            const int c = (tid % LANES) * 4;
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, join_m[w * ROWS + r]);
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) {
+                const float f = ex2(join_m[w * ROWS + r] - ref);
+                const float4 v = *reinterpret_cast<const float4*>(join_o + (w * ROWS + r) * Shape::kJoinStride + c);
+                sum = fmaf(f, join_l[w * ROWS + r], sum);
+                acc.x = fmaf(f, v.x, acc.x);
+                acc.y = fmaf(f, v.y, acc.y);
+                acc.z = fmaf(f, v.z, acc.z);
+                acc.w = fmaf(f, v.w, acc.w);
+            }
+            if (begins && ends) {
+                write_row<T>(a, it, r, c, acc, sum);
+            } else {
+                *reinterpret_cast<float4*>(&block->o[r][c]) = acc;
+                if (c == 0) {
+                    block->m[r] = top;
+                    block->l[r] = sum;
+                }
+            }
+        }
+        at += t_end - share.t;
+        if (begins && !ends && tid == 0)
+            a.joins[blockIdx.x] = make_int4(it.b, it.rt, it.h, owner(share, at + (it.tiles - t_end) - 1));
+        if (at >= share.end || !next_item<ROWS, kRowsKeys>(a, it)) return;
+        share.t = 0;
+        __syncthreads();  // before the rings and the rows are filled again
+    }
+}
+
+}  // namespace ako_b200

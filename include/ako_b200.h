@@ -1,6 +1,7 @@
 /*
  * ako_b200.h — C ABI of the B200 (sm_100a) kernels for AKO's memory-bound
- * inference operators: RMSNorm, fused residual-add RMSNorm, RoPE and SwiGLU.
+ * inference operators: RMSNorm, fused residual-add RMSNorm, RoPE and SwiGLU,
+ * and of the paged key/value cache that a decoder keeps next to them.
  *
  * Every entry point takes plain device pointers, element strides and sizes, a
  * dtype code and a CUDA stream passed as `void*` (a `cudaStream_t`; NULL is
@@ -40,7 +41,8 @@ extern "C" {
 typedef enum {
     AKO_B200_F32 = 0,
     AKO_B200_F16 = 1,
-    AKO_B200_BF16 = 2
+    AKO_B200_BF16 = 2,
+    AKO_B200_E4M3 = 3 /* only as the element type of a paged cache */
 } ako_b200_dtype;
 
 typedef enum {
@@ -243,6 +245,121 @@ int ako_b200_rope_plan(int64_t batch, int64_t seq_len, int64_t n_heads, int64_t 
  */
 int ako_b200_swiglu_plan(int64_t n_rows, int64_t hidden_dim, int dtype, int aligned, int dense,
                          int* access_bytes, int* threads, int* vectors_per_thread, int* threads_per_sm);
+
+/* ------------------------------------------------------------------------
+ * Paged key/value cache. The reference keeps a dense cache that it
+ * concatenates at every step (ako/models/decoder.py:84-93) and has no
+ * counterpart of what follows.
+ *
+ * One layer's cache: k and v are (num_pages, kv_heads, page_size, head_dim)
+ * with free element strides for the first three axes; the last is contiguous.
+ * dtype is that of the activations, or AKO_B200_E4M3 with one fp32 scale per
+ * token and head in k_scale and v_scale, (num_pages, kv_heads, page_size) with
+ * free strides: a cached value stands for element * scale. Scales are
+ * positive. k, v and all their strides are multiples of 16 bytes, head_dim a
+ * multiple of 8 (of 16 in an e4m3 cache) and at most 128.
+ */
+typedef struct {
+    void* k;
+    void* v;
+    float* k_scale; /* NULL unless dtype is AKO_B200_E4M3 */
+    float* v_scale;
+    int64_t k_stride_page, k_stride_head, k_stride_slot;
+    int64_t v_stride_page, v_stride_head, v_stride_slot;
+    int64_t ks_stride_page, ks_stride_head, ks_stride_slot;
+    int64_t vs_stride_page, vs_stride_head, vs_stride_slot;
+    int64_t num_pages, kv_heads, page_size, head_dim;
+    int64_t dtype;
+} ako_b200_paged_kv;
+
+/*
+ * The sequences of a step. Position p of sequence b lies in page
+ * page_table[b * page_table_stride + p / page_size], at offset p % page_size.
+ * kv_lens[b] tokens of it are cached, the step's new ones included. The new
+ * tokens of sequence b are its last positions: the rows cu_seqlens[b] up to
+ * cu_seqlens[b + 1] of the step's tokens, or, where cu_seqlens is NULL, the
+ * rows [b] of tensors that give every sequence the same number.
+ *
+ * All of it is device data that no entry point reads on the host, so that a
+ * captured graph can be replayed on new contents. Lengths are clamped to the
+ * table's extent (max_pages * page_size) and to the tokens given; a page number
+ * outside the cache, which may also stand for pages that a window has left
+ * behind, is a page that is not there: its positions are not written, read as
+ * zeros and attended by nobody. Rows behind cu_seqlens[batch] are left as
+ * they are.
+ */
+typedef struct {
+    const int32_t* page_table;
+    const int32_t* kv_lens;    /* batch */
+    const int32_t* cu_seqlens; /* batch + 1, or NULL */
+    int64_t page_table_stride;
+    int64_t batch, max_pages;
+    int64_t max_q_len; /* most new tokens of a sequence; sizes the launch, bounds nothing */
+} ako_b200_paged_batch;
+
+/*
+ * Stores the new tokens' keys and values in the cache. k and v: with
+ * cu_seqlens, `tokens` rows (stride_b is not used); without, batch x q_len
+ * rows, tokens = batch * q_len. Each row is kv_heads x head_dim, its last axis
+ * contiguous. A token at a position before 0 (a sequence of fewer cached than
+ * new tokens) is not stored. No two tokens of a call may share a slot.
+ *
+ * An e4m3 cache takes round(x / s) to nearest even, where s, the scale stored
+ * with it, is the least power of two with max|x| / s <= 448 over the token's
+ * finite values in the head (1 where they are all zero; at least 2^-126).
+ * Both x / s and element * s are then exact, so the one rounding is that to
+ * e4m3. Infinities are stored as +-448, NaN as NaN.
+ */
+int ako_b200_kv_cache_write(const void* k, int64_t k_stride_b, int64_t k_stride_s, int64_t k_stride_h,
+                            const void* v, int64_t v_stride_b, int64_t v_stride_s, int64_t v_stride_h,
+                            const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,
+                            int64_t tokens, int64_t q_len, int dtype, void* stream);
+
+/*
+ * Reads positions start .. start + length - 1 of every sequence into dense
+ * (batch, kv_heads, length, head_dim) outputs of `dtype` (that of the cache
+ * unless it is e4m3), with free strides for the first three axes. Positions
+ * behind a sequence's last are zero. An e4m3 cache's element * scale is
+ * rounded once. cu_seqlens is not used.
+ */
+int ako_b200_kv_cache_read(const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,
+                           int64_t start, int64_t length,
+                           void* k_out, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                           void* v_out, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
+                           int dtype, void* stream);
+
+/*
+ * Attention of the new tokens over the cache, which holds them already:
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / (q_heads / kv_heads)]) v[j, ...]
+ * over the keys j that token i, at position p, sees: j <= p, and with a
+ * window w > 0 only j > p - w or j < sinks. A row that sees none is zero.
+ * q and out are laid out as ako_b200_kv_cache_write's k and v, with q_heads
+ * heads, in fp16 or bf16 (`dtype`). Scores, the softmax's maximum and sum and
+ * the output's sum are fp32; the weights are rounded to the operands' 16-bit
+ * type for the second product, the output once.
+ *
+ * workspace: device memory of at least the bytes that
+ * ako_b200_paged_attention_plan reports, 16-byte aligned, used by this call
+ * alone until it has run (a captured call: by its graph alone).
+ */
+int ako_b200_paged_attention(const void* q, int64_t q_stride_b, int64_t q_stride_s, int64_t q_stride_h,
+                             const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,
+                             int64_t tokens, int64_t q_len, int64_t q_heads,
+                             double scale, int64_t window, int64_t sinks,
+                             void* out, int64_t out_stride_b, int64_t out_stride_s, int64_t out_stride_h,
+                             void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * The kernel that a call with these arguments would run on the current device
+ * (on 148 SMs where there is none), without launching anything and without
+ * reading device memory: *kernel 0 is the one for few rows (warp-level matrix
+ * instructions, *tile_rows rows of one sequence and kv head at a time), and
+ * its grid of *ctas CTAs shares the sequences' key tiles out evenly, whatever
+ * their lengths. *workspace_bytes: what ako_b200_paged_attention needs.
+ */
+int ako_b200_paged_attention_plan(const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,
+                                  int64_t tokens, int64_t q_len, int64_t q_heads, int dtype,
+                                  int* kernel, int* tile_rows, int* ctas, int64_t* workspace_bytes);
 
 #ifdef __cplusplus
 }
