@@ -1,5 +1,5 @@
 // Status and error reporting of the C ABI (declared in include/ako_b200.h),
-// and the host-mapped status word of the persistent kernels.
+// and the host-mapped status word of the kernels that wait.
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -54,8 +54,8 @@ int refuse_if_wait_expired(const char* op) {
     const int* w = g_status_word.load(std::memory_order_acquire);
     if (w == nullptr || *reinterpret_cast<const volatile int*>(w) == 0) return AKO_B200_OK;
     return set_error(AKO_B200_ERR_WAIT_EXPIRED,
-                     "%s: refused: a bounded wait for a bulk copy ran out in an earlier RMSNorm launch (its "
-                     "unwritten rows hold NaN); ako_b200_take_device_status reports and clears it",
+                     "%s: refused: a bounded wait ran out in an earlier RMSNorm or attention launch (its unwritten "
+                     "rows hold NaN); ako_b200_take_device_status reports and clears it",
                      op);
 }
 

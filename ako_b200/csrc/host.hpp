@@ -37,12 +37,16 @@ int sm_count();
 // Whether launches carry programmatic stream serialization (see launch_ex).
 bool pdl_enabled();
 
-// Host-mapped status word of the persistent RMSNorm kernels, allocated
+// Host-mapped status word of the kernels that wait (the persistent RMSNorm
+// kernels and attention on the tensor cores), allocated
 // (pinned, mapped, portable to every device) on first use; nullptr if that
 // allocation failed, with the error recorded. A kernel whose bounded wait
-// for a bulk copy runs out stores kStatusWaitTimeout there with a plain
+// runs out stores kStatusWaitTimeout there with a plain
 // system-scope store; the host reads it without synchronizing.
 int* device_status_word();
+
+// Polls that a kernel's bounded wait makes before it gives up (about a second).
+uint32_t wait_polls();
 
 // AKO_B200_ERR_WAIT_EXPIRED (with a message naming `op`) while the status
 // word holds an unreported expiry, else AKO_B200_OK. Every entry point that

@@ -9,6 +9,9 @@
 namespace ako_b200 {
 namespace {
 
+// Rows per sequence and kv head up to which the kernel for few rows runs.
+constexpr int kFewRows = 32;
+
 // Checks that need no pointer of the call; fills the sizes of `a`.
 int check_sizes(const char* op, const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch, int64_t tokens,
                 int64_t q_len, int64_t q_heads, int dtype, AttnArgs& a, AttnPlan& p) {
@@ -31,7 +34,13 @@ int check_sizes(const char* op, const ako_b200_paged_kv* cache, const ako_b200_p
     p.dtype = dtype;
     p.quant = cache->dtype == AKO_B200_E4M3;
     p.wide = a.cache.head_dim > 64;
-    make_plan(most * a.group, p);
+    const int64_t rows = most * a.group;
+    if (rows <= kFewRows) {
+        p.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+        plan_rows(p);
+    } else {
+        plan_tiles(p);
+    }
     return AKO_B200_OK;
 }
 
@@ -87,7 +96,8 @@ extern "C" int ako_b200_paged_attention(const void* q, int64_t q_stride_b, int64
     a.scale = static_cast<float>(scale * 1.4426950408889634);
     a.joins = static_cast<int4*>(workspace);
     a.partial = reinterpret_cast<float*>(a.joins + p.ctas);
-    return launch_attention(a, p, static_cast<cudaStream_t>(stream));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return p.kernel == 0 ? launch_rows(a, p, st) : launch_tiles(a, p, scale, st);
 }
 
 extern "C" int ako_b200_paged_attention_plan(const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,

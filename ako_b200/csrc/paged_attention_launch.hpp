@@ -12,10 +12,32 @@ struct AttnPlan {
     int64_t workspace;  // bytes: an int4 per CTA, then two partial blocks per CTA
 };
 
-// Fills kernel, tile_rows, ctas and workspace for calls whose longest
-// sequence has `rows` rows (new tokens times q heads) per kv head.
-void make_plan(int64_t rows, AttnPlan& p);
+// Raises a kernel's limit of dynamic shared memory once per device.
+template <typename K>
+int allow_smem(K kernel, int bytes, bool (&done)[64], const char* name) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (done[dev]) return AKO_B200_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(AKO_B200_ERR_CUDA, "%s: %d bytes of shared memory: %s", name, bytes, cudaGetErrorString(e));
+    }
+    done[dev] = true;
+    return AKO_B200_OK;
+}
 
-int launch_attention(const AttnArgs& a, const AttnPlan& p, cudaStream_t st);
+// Bytes of workspace for `ctas` CTAs that keep blocks of `rows` rows.
+inline int64_t attention_workspace(int ctas, int rows, bool wide) {
+    return static_cast<int64_t>(ctas) * (sizeof(int4) + 2 * sizeof(float) * rows * (2 + (wide ? 128 : 64)));
+}
+
+// Kernel 0, for few rows: tile_rows is 8, 16 or 32.
+void plan_rows(AttnPlan& p);
+int launch_rows(const AttnArgs& a, const AttnPlan& p, cudaStream_t st);
+
+// Kernel 1, on the tensor cores; `scale` is the call's, with its sign.
+void plan_tiles(AttnPlan& p);
+int launch_tiles(const AttnArgs& a, const AttnPlan& p, double scale, cudaStream_t st);
 
 }  // namespace ako_b200

@@ -5,21 +5,6 @@
 namespace ako_b200 {
 namespace {
 
-// Raises a kernel's limit of dynamic shared memory once per device.
-template <typename K>
-int allow_smem(K kernel, int bytes, bool (&done)[64], const char* name) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (done[dev]) return AKO_B200_OK;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return set_error(AKO_B200_ERR_CUDA, "%s: %d bytes of shared memory: %s", name, bytes, cudaGetErrorString(e));
-    }
-    done[dev] = true;
-    return AKO_B200_OK;
-}
-
 template <typename T, bool QUANT, int DPAD, int NT>
 int launch(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
     using Shape = RowsShape<T, QUANT, DPAD, NT>;
@@ -38,12 +23,12 @@ template <typename T, bool QUANT, int DPAD, int NT>
 void plan(AttnPlan& p) {
     using Shape = RowsShape<T, QUANT, DPAD, NT>;
     p.kernel = 0;
-    p.tile_rows = Shape::kRows;
     p.ctas = sm_count() * Shape::kCtas;
-    p.workspace = static_cast<int64_t>(p.ctas) * (sizeof(int4) + 2 * sizeof(PartialBlock<Shape::kRows, DPAD>));
+    p.workspace = attention_workspace(p.ctas, Shape::kRows, DPAD == 128);
+    static_assert(sizeof(PartialBlock<Shape::kRows, DPAD>) == sizeof(float) * Shape::kRows * (2 + DPAD), "block size");
 }
 
-// f.template operator()<T, QUANT, DPAD, NT>() for the instantiation of `p`.
+// f.run<T, QUANT, DPAD, NT>() for the instantiation of `p`.
 template <typename T, bool QUANT, int DPAD, typename F>
 int with_rows(const AttnPlan& p, F f) {
     switch (p.tile_rows) {
@@ -85,11 +70,8 @@ struct Launch {
 
 }  // namespace
 
-void make_plan(int64_t rows, AttnPlan& p) {
-    p.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-    with_plan(p, Plan{p});
-}
+void plan_rows(AttnPlan& p) { with_plan(p, Plan{p}); }
 
-int launch_attention(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) { return with_plan(p, Launch{a, p, st}); }
+int launch_rows(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) { return with_plan(p, Launch{a, p, st}); }
 
 }  // namespace ako_b200

@@ -305,6 +305,9 @@ int check_operand(const char* op, const char* name, const void* p, int64_t strid
 }
 
 }  // namespace
+
+uint32_t wait_polls() { return g_wait_polls; }
+
 }  // namespace ako_b200
 
 using namespace ako_b200;
