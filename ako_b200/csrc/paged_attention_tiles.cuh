@@ -3,14 +3,15 @@
 //
 // A CTA holds 256 rows of one sequence and kv head (new tokens times the q
 // heads that share it) as two halves of 128 and goes over the keys in tiles of
-// 128, one CTA per SM. The scores S = Q K^T of a half go to tensor memory; its
-// four warps, a row to a thread, take them from there, write the weights P
-// over them in 16 bits, and O += P V reads P from tensor memory. While one
-// half's warps work on their softmax the tensor cores work for the other:
+// 128, one CTA per SM. The scores S = Q K^T of a half and 64 keys go to tensor
+// memory; the half's four warps, a row to a thread, take them from there, write
+// the weights P over them in 16 bits, and O += P V reads P from tensor memory.
+// Each half has two such strips of 64 scores, so that its warps always have
+// one to work on while the tensor cores turn the other from P into the next S:
 //
-//   tensor cores  | O_a += P_a V, S_a | O_b += P_b V, S_b | O_a += ...
-//   half a's warps|                   | softmax of S_a    |
-//   half b's warps| softmax of S_b    |                   | softmax of S_b
+//   tensor cores  | O_a += P_a0 V, S_a0 | O_b += P_b0 V, S_b0 | O_a += P_a1 V, S_a1 | ...
+//   half a's warps| softmax of S_a1 ...       | softmax of S_a0 ...
+//   half b's warps| softmax of S_b1 ...             | softmax of S_b0 ...
 //
 // Four more warps bring keys and values into shared memory (rows anywhere in
 // the cache, swizzled for the products), and one thread issues the products.
@@ -35,10 +36,10 @@ namespace ako_b200 {
 constexpr int kTilesThreads = 512;
 constexpr int kTilesRows = 256;
 constexpr int kTilesKeys = 128;
+constexpr int kStrip = 64;  // keys of a strip of scores
 // Tiles whose key data are kept: the loading warps find a tile's keys one tile
 // before they bring them, at most STAGES + 2 tiles ahead of the softmax.
 constexpr int kMetaStages = 8;
-constexpr int kOffsetStages = 4;
 constexpr uint32_t kDrainLimit = 1u << 24;
 // Registers per thread of the softmax, loading and issuing warps. The block is
 // launched with 128 a thread, and 2 * 184 + 96 + 48 = 4 * 128.
@@ -68,9 +69,9 @@ struct TileMeta {
 template <int STAGES>
 struct TilesShared {
     TileMeta meta[kMetaStages];
-    int64_t offset[kOffsetStages][2][kTilesKeys];  // of the keys' rows in k and v, or -1
     uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2], o_full[2], drained;
+    uint4 staging[8][128];  // of a softmax warp: 32 rows of 64 bytes on their way out
     uint32_t tmem;
     volatile int stop;     // a wait ran out
     volatile int odd;      // a value that is not finite was taken out of a tile that not every row sees
@@ -92,6 +93,11 @@ __device__ __forceinline__ bool tile_wait(S& sm, uint64_t* bar, uint32_t phase, 
 __device__ __forceinline__ bool whole_tile(const AttnArgs& a, const Item& it, int key0) {
     return key0 + kTilesKeys - 1 <= it.p_lo &&
            (a.window == 0 || key0 > it.p_hi - a.window || key0 + kTilesKeys <= a.sinks);
+}
+
+// The same for a strip.
+__device__ __forceinline__ bool whole_strip(const AttnArgs& a, const Item& it, int key0) {
+    return key0 + kStrip - 1 <= it.p_lo && (a.window == 0 || key0 > it.p_hi - a.window || key0 + kStrip <= a.sinks);
 }
 
 __device__ __forceinline__ bool sees_key(const AttnArgs& a, int pos, int key) {
@@ -143,87 +149,112 @@ __device__ __forceinline__ bool scrub(uint4& v) {
     return any != 0;
 }
 
+// One of the four loading warps, which brings 32 keys of every tile. A lane
+// looks after one key's place in the cache and copies chunks of several rows.
 template <typename T, bool QUANT, int DPAD>
 struct TileLoader {
-    using Shape = TilesShape<DPAD>;
-    using Shared = TilesShared<Shape::kStages>;
     static constexpr int ES = QUANT ? 1 : 2;
-    static constexpr int CHUNKS = DPAD * ES / 16;      // 16-byte chunks of a cached row
-    static constexpr int ROWS = 128 / CHUNKS;          // rows that the 128 threads take at once
-    static constexpr int EACH = kTilesKeys / ROWS;     // chunks of a thread
+    static constexpr int CHUNKS = DPAD * ES / 16;  // 16-byte chunks of a cached row
+    static constexpr int ROWS = 32 / CHUNKS;       // rows that the warp takes at once
+    static constexpr int EACH = 32 / ROWS;         // chunks of a lane
     const AttnArgs& a;
-    Shared& sm;
-    int tid, chunk, row0;
+    int warp, lane, chunk, row0;
     bool real;  // the chunk lies within head_dim
 
-    __device__ TileLoader(const AttnArgs& args, Shared& shared, int t)
-        : a(args), sm(shared), tid(t), chunk(t % CHUNKS), row0(t / CHUNKS), real(chunk * 16 < args.cache.head_dim * ES) {}
+    // A key's place, as far as it is known: its table entry is on the way.
+    struct Place {
+        int page, slot, h;
+        bool whole;  // of the tile
+    };
+    // Where its row is.
+    struct Rows {
+        int64_t k, v;  // offsets, or -1
+        float ks, vs;
+        bool whole;
+    };
+
+    __device__ TileLoader(const AttnArgs& args, int w, int l)
+        : a(args), warp(w), lane(l), chunk(l % CHUNKS), row0(l / CHUNKS), real(chunk * 16 < args.cache.head_dim * ES) {}
 
     // Where the 16-bit chunk c of a row goes in a tile.
     static __device__ __forceinline__ uint32_t place(int row, int c) {
         return static_cast<uint32_t>((c >> 3) * (kTilesKeys * 128) + row * 128 + ((c & 7) ^ (row & 7)) * 16);
     }
 
-    // Finds the rows of a tile's keys and fills its meta data; every thread looks after one key.
-    __device__ __forceinline__ void find(const Item& it, int key0, int64_t (&offset)[2][kTilesKeys], TileMeta& meta) {
-        const int key = key0 + tid;
-        int page = -1, slot = 0;
-        if (key <= it.p_hi && (key >= it.win_lo || key < a.sinks)) page = page_of(a.seqs, a.cache, it.b, key, slot);
-        offset[0][tid] = page >= 0 ? a.cache.k.offset(page, it.h, slot) : -1;
-        offset[1][tid] = page >= 0 ? a.cache.v.offset(page, it.h, slot) : -1;
-        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-        if ((tid & 31) == 0) meta.there[tid >> 5] = there;
-        if constexpr (QUANT) {
-            float ks = 0.0f, vs = 1.0f;
-            if (page >= 0) {
-                ks = static_cast<const float*>(a.cache.ks.p)[a.cache.ks.offset(page, it.h, slot)];
-                vs = fmaxf(static_cast<const float*>(a.cache.vs.p)[a.cache.vs.offset(page, it.h, slot)], 0x1p-100f);
-            }
-            meta.kc[tid] = ks * a.scale;
-            meta.lv[tid] = __log2f(vs);
-            meta.unscale[tid] = __fdividef(1.0f, vs);
+    __device__ __forceinline__ Place look_up(const Item& it, int key0) const {
+        Place p{-1, 0, it.h, whole_tile(a, it, key0)};
+        const int key = key0 + warp * 32 + lane;
+        if (key <= it.p_hi && (key >= it.win_lo || key < a.sinks)) {
+            const int i = static_cast<int>(a.cache.by_page.div(static_cast<uint32_t>(key)));
+            p.slot = key - i * a.cache.page_size;
+            p.page = a.seqs.table[it.b * a.seqs.table_stride + i];
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        return p;
+    }
+
+    __device__ __forceinline__ Rows find(const Place& p, TileMeta& meta) const {
+        Rows r{-1, -1, 0.0f, 1.0f, p.whole};
+        const bool there = p.page >= 0 && p.page < a.cache.num_pages;
+        if (there) {
+            r.k = a.cache.k.offset(p.page, p.h, p.slot);
+            r.v = a.cache.v.offset(p.page, p.h, p.slot);
+            if constexpr (QUANT) {
+                r.ks = static_cast<const float*>(a.cache.ks.p)[a.cache.ks.offset(p.page, p.h, p.slot)];
+                r.vs = static_cast<const float*>(a.cache.vs.p)[a.cache.vs.offset(p.page, p.h, p.slot)];
+            }
+        }
+        const unsigned bits = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) meta.there[warp] = bits;
+        return r;
+    }
+
+    // An e4m3 cache's scales, as the kernel for few rows has them.
+    __device__ __forceinline__ void put_scales(const Rows& r, TileMeta& meta) const {
+        const float vs = fmaxf(r.vs, 0x1p-100f);
+        meta.kc[warp * 32 + lane] = r.ks * a.scale;
+        meta.lv[warp * 32 + lane] = __log2f(vs);
+        meta.unscale[warp * 32 + lane] = __fdividef(1.0f, vs);
     }
 
     // 16-bit caches: copies straight into the tile.
-    __device__ __forceinline__ void copy(const void* base, const int64_t* offset, uint32_t tile) const {
+    __device__ __forceinline__ void copy(const void* base, int64_t offset, uint32_t tile) const {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int row = row0 + i * ROWS;
-            const int64_t o = offset[row];
+            const int64_t o = __shfl_sync(0xffffffffu, offset, row);
             const bool there = o >= 0 && real;
-            cp_async16_or_zero(tile + place(row, chunk),
+            cp_async16_or_zero(tile + place(warp * 32 + row, chunk),
                                there ? static_cast<const uint8_t*>(base) + (o + chunk * 8) * 2 : base, there);
         }
     }
 
-    // Takes what is not finite out of this thread's chunks of a tile of values.
-    __device__ __forceinline__ void scrub_copied(uint8_t* tile) {
+    // Takes what is not finite out of this lane's chunks of a tile of values.
+    __device__ __forceinline__ bool scrub_copied(uint8_t* tile) const {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            uint4* const p = reinterpret_cast<uint4*>(tile + place(row0 + i * ROWS, chunk));
+            uint4* const p = reinterpret_cast<uint4*>(tile + place(warp * 32 + row0 + i * ROWS, chunk));
             uint4 v = *p;
             if (scrub<T>(v)) {
                 *p = v;
                 any = true;
             }
         }
-        if (any) sm.odd = 1;
+        return any;
     }
 
     // e4m3 caches: into registers, and from there as fp16.
-    __device__ __forceinline__ void fetch(const void* base, const int64_t* offset, uint4 (&v)[EACH]) const {
+    __device__ __forceinline__ void fetch(const void* base, int64_t offset, uint4 (&v)[EACH]) const {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int64_t o = offset[row0 + i * ROWS];
+            const int64_t o = __shfl_sync(0xffffffffu, offset, row0 + i * ROWS);
             v[i] = make_uint4(0, 0, 0, 0);
             if (o >= 0 && real) v[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + o + chunk * 16);
         }
     }
 
-    __device__ __forceinline__ void convert(const uint4 (&v)[EACH], uint8_t* tile, bool clean) {
+    // True if `clean` took anything out.
+    __device__ __forceinline__ bool convert(const uint4 (&v)[EACH], uint8_t* tile, bool clean) const {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
@@ -233,12 +264,18 @@ struct TileLoader {
                 uint4 w = make_uint4(e4m3x2_to_half2(u[2 * half]), e4m3x2_to_half2(u[2 * half] >> 16),
                                      e4m3x2_to_half2(u[2 * half + 1]), e4m3x2_to_half2(u[2 * half + 1] >> 16));
                 if (clean && scrub<__half>(w)) any = true;
-                *reinterpret_cast<uint4*>(tile + place(row0 + i * ROWS, chunk * 2 + half)) = w;
+                *reinterpret_cast<uint4*>(tile + place(warp * 32 + row0 + i * ROWS, chunk * 2 + half)) = w;
             }
         }
-        if (any) sm.odd = 1;
+        return any;
     }
 };
+
+// Bits 32 w .. 32 w + 31 of the mask whose first `n` bits (none if negative) are set.
+__device__ __forceinline__ uint32_t first_bits(int n, int w) {
+    const int k = min(max(n - 32 * w, 0), 32);
+    return k == 32 ? 0xffffffffu : (1u << k) - 1u;
+}
 
 template <typename T, bool QUANT, int DPAD>
 __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const TilesArgs args) {
@@ -256,7 +293,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
     uint8_t* const q_tile = tiles;                        // two halves
     uint8_t* const k_tile = tiles + 2 * Shape::kOperand;  // STAGES of keys, then of values
     uint8_t* const v_tile = k_tile + STAGES * Shape::kOperand;
-    const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31, wg = tid >> 7;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), wg = warp >> 2;
     const uint32_t polls = args.wait_polls;
 
     if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -271,9 +309,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
         }
         for (int h = 0; h < 2; ++h) {
             mbar_init(&sm.q_full[h], 128);
-            mbar_init(&sm.s_full[h], 1);
-            mbar_init(&sm.p_full[h], 128);
+            mbar_init(&sm.o_done[h], 1);
             mbar_init(&sm.o_full[h], 1);
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&sm.s_full[h][j], 1);
+                mbar_init(&sm.p_full[h][j], 128);
+            }
         }
         mbar_init(&sm.drained, 1);
         fence_mbar_init();
@@ -298,201 +339,224 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
     if (wg == 3) {
         // ---------------------------------------------------------- products
         give_registers<kIssueRegs>();
-        if (warp == 12 && lane == 0) {
-            const int steps = (a.cache.head_dim + 15) / 16;
-            const uint32_t s_shape = mma_shape(128, kTilesKeys, TYPE, false);
-            const uint32_t o_shape = mma_shape(128, steps * 16, TYPE, true);
-            constexpr uint32_t BLOCK = kTilesKeys * 128;  // bytes of 64 columns of a tile
-            const uint32_t q_addr = smem_addr(q_tile), k_addr = smem_addr(k_tile), v_addr = smem_addr(v_tile);
-            uint32_t n = 0;            // tiles so far
-            uint32_t ns[2] = {0, 0};   // of a half
-            uint32_t nq[2] = {0, 0};   // items of a half
-            bool ok = true;
-            auto weigh = [&](int h, uint32_t tile, bool add) {  // O_h (+)= P_h V
-                ok = ok && tile_wait(sm, &sm.p_full[h], (ns[h] - 1) & 1, polls);
-                ok = ok && tile_wait(sm, &sm.v_full[tile % STAGES], (tile / STAGES) & 1, polls);
-                if (!ok) return;
-                tmem_fence_after();
-                const uint32_t v = v_addr + (tile % STAGES) * Shape::kOperand;
+        if (warp != 12) return;
+        // The whole warp follows the loop, so that addresses and descriptors are uniform; one
+        // elected lane issues the products and commits them.
+        const bool leader = elect_one();
+        const int steps = (a.cache.head_dim + 15) / 16;
+        const uint32_t s_shape = mma_shape(128, kStrip, TYPE, false);
+        const uint32_t o_shape = mma_shape(128, steps * 16, TYPE, true);
+        constexpr uint32_t BLOCK = kTilesKeys * 128;  // bytes of 64 columns of a tile
+        // a descriptor's address counts 16 bytes
+        const uint64_t q_desc = smem_operand(smem_addr(q_tile), 16), k_desc = smem_operand(smem_addr(k_tile), 16);
+        const uint64_t v_desc = smem_operand(smem_addr(v_tile), BLOCK);
+        uint32_t n = 0;           // tiles so far
+        uint32_t ns[2] = {0, 0};  // of a half
+        uint32_t nq[2] = {0, 0};  // items of a half
+        bool ok = true;
+        auto await = [&](uint64_t* bar, uint32_t phase) {
+            ok = ok && tile_wait(sm, bar, phase & 1, polls);
+            ok = __all_sync(0xffffffffu, ok);
+            return ok;
+        };
+        // O_h (+)= P_h V of strip j of the half's tile `mine`, the CTA's tile `tile`
+        auto weigh = [&](int h, int j, uint32_t mine, uint32_t tile, bool add) {
+            if (!await(&sm.p_full[h][j], mine)) return;
+            if (j == 0 && h == 0) {
+                if (!await(&sm.v_full[tile % STAGES], tile / STAGES)) return;
+                fence_proxy_async_smem();  // the copies were not this proxy's
+            }
+            tmem_fence_after();
+            const uint64_t v = v_desc + ((tile % STAGES) * Shape::kOperand + j * kStrip * 128) / 16;
+            const uint32_t o = tmem + O_COL + h * 128, p = tmem + h * 128 + j * kStrip;
+            if (leader) {
 #pragma unroll
-                for (int k = 0; k < kTilesKeys / 16; ++k)
-                    mma_ts(tmem + O_COL + h * 128, tmem + h * 128 + k * 8, smem_operand(v + k * 16 * 128, BLOCK), o_shape,
-                           add || k > 0);
-            };
-            do {
-                const int t_end = part_end();
-                const int halves = it.rows > 128 ? 2 : 1;
-                for (int t = share.t; t < t_end && ok; ++t, ++n) {
-                    ok = ok && tile_wait(sm, &sm.k_full[n % STAGES], (n / STAGES) & 1, polls);
-                    for (int h = 0; h < halves && ok; ++h) {
-                        if (t == share.t) {
-                            ok = tile_wait(sm, &sm.q_full[h], nq[h] & 1, polls);
-                            ++nq[h];
-                        } else {
-                            weigh(h, n - 1, t - 1 > share.t);
-                            if (h == halves - 1) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
-                        }
+                for (int k = 0; k < kStrip / 16; ++k) mma_ts(o, p + k * 8, v + k * (16 * 128 / 16), o_shape, add || k > 0);
+                mma_commit(&sm.o_done[h]);
+            }
+        };
+        do {
+            const int t_end = part_end();
+            const int halves = it.rows > 128 ? 2 : 1;
+            for (int t = share.t; t < t_end && ok; ++t, ++n) {
+                await(&sm.k_full[n % STAGES], n / STAGES);
+                fence_proxy_async_smem();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h >= halves || !ok) break;
+                        if (t > share.t) weigh(h, j, ns[h] - 1, n - 1, j > 0 || t - 1 > share.t);
+                        else if (j == 0) await(&sm.q_full[h], nq[h]++);
                         if (!ok) break;
                         tmem_fence_after();
-                        const uint32_t q = q_addr + h * Shape::kOperand, k = k_addr + (n % STAGES) * Shape::kOperand;
-                        for (int s = 0; s < steps; ++s) {
-                            const uint32_t to = (s >> 2) * BLOCK + (s & 3) * 32;
-                            mma_ss(tmem + h * 128, smem_operand(q + to, 16), smem_operand(k + to, 16), s_shape, s > 0);
+                        const uint64_t q = q_desc + h * Shape::kOperand / 16;
+                        const uint64_t k = k_desc + ((n % STAGES) * Shape::kOperand + j * kStrip * 128) / 16;
+                        if (leader) {
+#pragma unroll
+                            for (int s = 0; s < DPAD / 16; ++s) {
+                                const uint32_t to = ((s >> 2) * BLOCK + (s & 3) * 32) / 16;
+                                if (s < steps) mma_ss(tmem + h * 128 + j * kStrip, q + to, k + to, s_shape, s > 0);
+                            }
+                            mma_commit(&sm.s_full[h][j]);
                         }
-                        ++ns[h];
-                        mma_commit(&sm.s_full[h]);
+                        if (j == 1) ++ns[h];
                     }
+                }
+                if (leader) {
+                    if (t > share.t) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
                     mma_commit(&sm.k_empty[n % STAGES]);
                 }
-                for (int h = 0; h < halves && ok; ++h) {
-                    weigh(h, n - 1, t_end - 1 > share.t);
-                    mma_commit(&sm.o_full[h]);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h >= halves || !ok) break;
+                    weigh(h, j, ns[h] - 1, n - 1, j > 0 || t_end - 1 > share.t);
+                    if (j == 1 && leader) mma_commit(&sm.o_full[h]);
                 }
-                mma_commit(&sm.v_empty[(n - 1) % STAGES]);
-                if (!advance(t_end)) break;
-            } while (ok);
-            // nothing of this CTA's is under way when it gives its tensor memory back
-            mma_commit(&sm.drained);
-            mbar_wait_bounded(&sm.drained, 0, kDrainLimit);
-        }
+            if (leader) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
+            if (!advance(t_end)) break;
+        } while (ok);
+        // nothing of this CTA's is under way when it gives its tensor memory back
+        if (leader) mma_commit(&sm.drained);
+        mbar_wait_bounded(&sm.drained, 0, kDrainLimit);
         __syncwarp();
+        // the other roles are done with tensor memory
+        asm volatile("bar.sync 2, 416;" ::: "memory");
+        tmem_fence_after();
+        if (lane == 0 && sm.stop) *reinterpret_cast<volatile int*>(args.status) = kStatusWaitTimeout;
+        tmem_free<512>(tmem);
     } else if (wg == 2) {
         // ----------------------------------------------------------- loading
         give_registers<kLoadRegs>();
-        TileLoader<T, QUANT, DPAD> load(a, sm, tid - 256);
+        using Loader = TileLoader<T, QUANT, DPAD>;
+        const Loader load(a, warp & 3, lane);
         const uint32_t k_addr = smem_addr(k_tile), v_addr = smem_addr(v_tile);
-        uint32_t n = 0;
         bool ok = true;
-        uint64_t* pending = nullptr;  // full barrier of the copies under way before the last
-        uint8_t* dirty = nullptr;     // their tile, if its values are to be cleaned
-        auto landed = [&] {
-            if (dirty != nullptr) load.scrub_copied(dirty);
-            fence_proxy_async_smem();
-            mbar_arrive(pending);
-            pending = nullptr;
-        };
-        // Waits until a stage is free, handing on first what has been copied.
         auto acquire = [&](uint64_t* empty, uint32_t use) {
-            const uint32_t phase = ((use / STAGES) & 1) ^ 1;
-            if (mbar_try_wait(empty, phase)) return;
-            if (pending != nullptr) {
-                cp_async_wait<0>();
-                landed();
-            }
-            ok = ok && tile_wait(sm, empty, phase, polls);
+            ok = ok && tile_wait(sm, empty, ((use / STAGES) & 1) ^ 1, polls);
+            ok = __all_sync(0xffffffffu, ok);
         };
-        auto issued = [&](uint64_t* full, uint8_t* clean) {
-            cp_async_commit();
-            if (pending != nullptr) {
-                cp_async_wait<1>();
-                landed();
-            }
-            pending = full;
-            dirty = clean;
-        };
-        // A tile's keys are found while the tile before is on its way.
+        // The table entries of a tile's keys are asked for two tiles ahead and its rows known one
+        // tile ahead, so that a tile waits for neither.
         int t_end = part_end();
         int t = share.t;
-        bool whole;
-        auto find = [&] {
-            const int key0 = key_tile(it, t) * kTilesKeys;
-            whole = whole_tile(a, it, key0);
-            load.find(it, key0, sm.offset[n % kOffsetStages], sm.meta[n % kMetaStages]);
-        };
-        auto next = [&] {
-            ++n;
+        bool last = false;  // nothing behind the tile looked up last
+        auto ahead = [&] {
             if (++t == t_end) {
-                if (!advance(t_end)) return false;
+                last = !advance(t_end);
                 t = 0;
-                t_end = part_end();
+                t_end = last ? 1 : part_end();
             }
-            find();
-            return true;
+            return last ? typename Loader::Place{-1, 0, 0, true} : load.look_up(it, key_tile(it, t) * kTilesKeys);
         };
-        find();
-        bool more = true;
-        [[maybe_unused]] uint4 kv[TileLoader<T, QUANT, DPAD>::EACH], vv[TileLoader<T, QUANT, DPAD>::EACH];
+        typename Loader::Rows rows = load.find(load.look_up(it, key_tile(it, t) * kTilesKeys), sm.meta[0]);
+        typename Loader::Place place = ahead();
+        bool more = !last;
+        [[maybe_unused]] uint4 kv[Loader::EACH], vv[Loader::EACH];
         if constexpr (QUANT) {
-            load.fetch(a.cache.k.p, sm.offset[0][0], kv);
-            load.fetch(a.cache.v.p, sm.offset[0][1], vv);
+            load.fetch(a.cache.k.p, rows.k, kv);
+            load.fetch(a.cache.v.p, rows.v, vv);
         }
-        while (more) {
+        for (uint32_t n = 0;; ++n) {
             const int st = n % STAGES;
-            const uint32_t use = n;
-            const bool clean = !whole;
+            const typename Loader::Rows now = rows;
             uint8_t* const vt = v_tile + st * Shape::kOperand;
-            acquire(&sm.k_empty[st], use);
+            const bool next = more;
+            acquire(&sm.k_empty[st], n);
             if (!ok) break;
-            if constexpr (!QUANT) {
-                load.copy(a.cache.k.p, sm.offset[use % kOffsetStages][0], k_addr + st * Shape::kOperand);
-                issued(&sm.k_full[st], nullptr);
-                more = next();
-                acquire(&sm.v_empty[st], use);
-                if (!ok) break;
-                load.copy(a.cache.v.p, sm.offset[use % kOffsetStages][1], v_addr + st * Shape::kOperand);
-                issued(&sm.v_full[st], clean ? vt : nullptr);
-            } else {
+            if constexpr (QUANT) {
+                load.put_scales(now, sm.meta[n % kMetaStages]);
                 load.convert(kv, k_tile + st * Shape::kOperand, false);
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.k_full[st]);
-                more = next();
-                if (more) load.fetch(a.cache.k.p, sm.offset[n % kOffsetStages][0], kv);
-                acquire(&sm.v_empty[st], use);
-                if (!ok) break;
-                load.convert(vv, vt, clean);
+            } else {
+                load.copy(a.cache.k.p, now.k, k_addr + st * Shape::kOperand);
+                mbar_arrive_copied(&sm.k_full[st]);
+            }
+            if (next) {
+                rows = load.find(place, sm.meta[(n + 1) % kMetaStages]);
+                if constexpr (QUANT) load.fetch(a.cache.k.p, rows.k, kv);
+                place = ahead();
+                more = !last;
+            }
+            acquire(&sm.v_empty[st], n);
+            if (!ok) break;
+            if constexpr (QUANT) {
+                if (load.convert(vv, vt, !now.whole)) sm.odd = 1;
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.v_full[st]);
-                if (more) load.fetch(a.cache.v.p, sm.offset[n % kOffsetStages][1], vv);
+                if (next) load.fetch(a.cache.v.p, rows.v, vv);
+            } else {
+                load.copy(a.cache.v.p, now.v, v_addr + st * Shape::kOperand);
+                if (now.whole) {
+                    mbar_arrive_copied(&sm.v_full[st]);
+                } else {
+                    cp_async_wait_everything();
+                    if (load.scrub_copied(vt)) sm.odd = 1;
+                    mbar_arrive(&sm.v_full[st]);
+                }
             }
+            if (!next) break;
         }
-        cp_async_wait<0>();
-        if (pending != nullptr) landed();
+        cp_async_wait_everything();
+        asm volatile("bar.arrive 2, 416;" ::: "memory");
     } else {
         // ----------------------------------------------------------- softmax
         take_registers<kSoftmaxRegs>();
-        const int h = wg, row = tid & 127;
+        const int h = wg, row = tid & 127, row0 = h * 128 + (warp & 3) * 32;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // first lane of the warp, in bits 16 up
         const uint32_t s_at = tmem + lanes + h * 128, o_at = tmem + lanes + O_COL + h * 128;
         uint8_t* const my_q = q_tile + h * Shape::kOperand;
-        uint32_t n = 0, ns = 0, no = 0;
+        uint4* const staging = sm.staging[warp];
+        uint32_t n = 0, ns = 0, no = 0;  // tiles of the CTA and of this half, and the half's items
         bool ok = true;
         int pos = 0;
         float factor = 1.0f;
-        // Brings this thread's row of q into the half's tile; `factor` takes out what it was scaled by.
+        // Brings the warp's rows of q into the half's tile, a row by DPAD / 8 lanes; `factor` takes
+        // out what this thread's row was scaled by.
         auto load_q = [&] {
-            const int r = h * 128 + row;
+            constexpr int LANES = DPAD / 8, TAKEN = 32 / LANES, TIMES = 32 / TAKEN;
+            const int r = row0 + lane, c = lane % LANES;
             const bool real = r < it.rows;
             pos = real ? it.kv - it.n + static_cast<int>(a.by_group.div(it.row0 + r)) : it.p_hi;
-            const T* const p = static_cast<const T*>(a.q) + (real ? row_offset(a, it, it.row0 + r, a.qb, a.qs, a.qh) : 0);
-            float top = 0.0f;
+            const int64_t mine = real ? row_offset(a, it, it.row0 + r, a.qb, a.qs, a.qh) : -1;
             factor = 1.0f;
-            float inv = args.q_factor;
-            if constexpr (QUANT && !std::is_same_v<T, __half>) {
-                if (real) {
-                    for (int c = 0; c < a.cache.head_dim; c += 8) {
-                        const Packed<T, 8> x = ld_cached<T, 8>(p + c);
+            Packed<T, 8> x[TIMES];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_f32(x.v[i])));
-                    }
-                }
-                if (top > 0.0f && top < INFINITY) {  // as in the kernel for few rows
-                    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 8, -126), 118);
-                    inv *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                    factor = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-                }
+            for (int i = 0; i < TIMES; ++i) {
+                const int64_t o = __shfl_sync(0xffffffffu, mine, i * TAKEN + lane / LANES);
+                *reinterpret_cast<uint4*>(&x[i]) = make_uint4(0, 0, 0, 0);
+                if (o >= 0 && c * 8 < a.cache.head_dim) x[i] = ld_cached<T, 8>(static_cast<const T*>(a.q) + o + c * 8);
             }
-#pragma unroll 4
-            for (int c = 0; c < DPAD / 8; ++c) {
-                Packed<M, 8> y;
-                Packed<T, 8> x;
-                *reinterpret_cast<uint4*>(&x) = make_uint4(0, 0, 0, 0);
-                if (real && c * 8 < a.cache.head_dim) x = ld_cached<T, 8>(p + c * 8);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float2 f = get2(x, i);
-                    put2(y, i, f.x * inv, f.y * inv);
+            for (int i = 0; i < TIMES; ++i) {
+                const int to = i * TAKEN + lane / LANES;
+                float inv = args.q_factor;
+                if constexpr (QUANT && !std::is_same_v<T, __half>) {
+                    float top = 0.0f, f = 1.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f32(x[i].v[e])));
+#pragma unroll
+                    for (int off = LANES / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                    if (top > 0.0f && top < INFINITY) {  // as in the kernel for few rows
+                        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 8, -126), 118);
+                        inv *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                        f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                    }
+                    const float g = __shfl_sync(0xffffffffu, f, (lane % TAKEN) * LANES);
+                    if (lane / TAKEN == i) factor = g;
                 }
-                *reinterpret_cast<uint4*>(my_q + TileLoader<T, QUANT, DPAD>::place(row, c)) = *reinterpret_cast<uint4*>(&y);
+                Packed<M, 8> y;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float2 f = get2(x[i], e);
+                    put2(y, e, f.x * inv, f.y * inv);
+                }
+                *reinterpret_cast<uint4*>(my_q + TileLoader<T, QUANT, DPAD>::place((warp & 3) * 32 + to, c)) =
+                    *reinterpret_cast<uint4*>(&y);
             }
             fence_proxy_async_smem();
             mbar_arrive(&sm.q_full[h]);
@@ -500,8 +564,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
         bool loaded = false;
         while (true) {
             const int t0 = share.t, t_end = part_end();
-            const bool mine = it.rows > h * 128;
-            if (!mine) {  // the other half's rows are all there are
+            if (it.rows <= h * 128) {  // the other half's rows are all there are
                 n += t_end - t0;
                 loaded = false;
                 if (!advance(t_end)) break;
@@ -509,87 +572,105 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
             }
             if (!loaded) load_q();
             // Warps without a row take part in the barriers alone.
-            const bool rows = h * 128 + (warp & 3) * 32 < it.rows;
+            const bool rows = row0 < it.rows;
+            const float scale = QUANT ? 1.0f : a.scale;
             float ref = -INFINITY, sum = 0.0f;
             for (int t = t0; t < t_end && ok; ++t, ++n, ++ns) {
-                const int key0 = key_tile(it, t) * kTilesKeys;
                 const TileMeta& meta = sm.meta[n % kMetaStages];
-                ok = tile_wait(sm, &sm.s_full[h], ns & 1, polls);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tmem_fence_after();
-                if (rows) {
-                    float x[kTilesKeys];
+#pragma unroll 1
+                for (int j = 0; j < 2; ++j) {
+                    const int key0 = key_tile(it, t) * kTilesKeys + j * kStrip;
+                    const uint32_t strip = s_at + j * kStrip;
+                    ok = tile_wait(sm, &sm.s_full[h][j], ns & 1, polls);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    if (rows) {
+                        float x[kStrip];
 #pragma unroll
-                    for (int c = 0; c < kTilesKeys; c += 32) tmem_load32(s_at + c, reinterpret_cast<uint32_t*>(x + c));
-                    tmem_wait_load();
-                    if constexpr (QUANT) {
+                        for (int c = 0; c < kStrip; c += 32) tmem_load32(strip + c, reinterpret_cast<uint32_t*>(x + c));
+                        tmem_wait_load();
+                        if constexpr (QUANT) {
 #pragma unroll
-                        for (int c = 0; c < kTilesKeys; c += 4) {
-                            const float4 kc = *reinterpret_cast<const float4*>(meta.kc + c);
-                            const float4 lv = *reinterpret_cast<const float4*>(meta.lv + c);
-                            x[c] = fmaf(x[c], kc.x * factor, lv.x);
-                            x[c + 1] = fmaf(x[c + 1], kc.y * factor, lv.y);
-                            x[c + 2] = fmaf(x[c + 2], kc.z * factor, lv.z);
-                            x[c + 3] = fmaf(x[c + 3], kc.w * factor, lv.w);
-                        }
-                    }
-                    const uint32_t there[4] = {meta.there[0], meta.there[1], meta.there[2], meta.there[3]};
-                    const bool full = (there[0] & there[1] & there[2] & there[3]) == 0xffffffffu;
-                    if (!full || !whole_tile(a, it, key0)) {
-#pragma unroll
-                        for (int c = 0; c < kTilesKeys; ++c)
-                            if ((there[c / 32] >> (c % 32) & 1) == 0 || !sees_key(a, pos, key0 + c)) x[c] = -INFINITY;
-                    }
-                    float top = x[0];
-#pragma unroll
-                    for (int c = 1; c < kTilesKeys; ++c) top = fmaxf(top, x[c]);
-                    const float scale = QUANT ? 1.0f : a.scale;
-                    top *= scale;
-                    const bool grew = top > ref + (ref == -INFINITY ? 0.0f : kGrowth);
-                    if (__any_sync(0xffffffffu, grew)) {
-                        const float to = grew ? top : ref;
-                        const float alpha = grew ? ex2(ref - to) : 1.0f;
-                        ref = to;
-                        sum *= alpha;
-                        if (t > t0) {
-#pragma unroll
-                            for (int c = 0; c < DPAD; c += 32) {
-                                uint32_t o[32];
-                                tmem_load32(o_at + c, o);
-                                tmem_wait_load();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                                tmem_store32(o_at + c, o);
+                            for (int c = 0; c < kStrip; c += 4) {
+                                const float4 kc = *reinterpret_cast<const float4*>(meta.kc + j * kStrip + c);
+                                const float4 lv = *reinterpret_cast<const float4*>(meta.lv + j * kStrip + c);
+                                x[c] = fmaf(x[c], kc.x * factor, lv.x);
+                                x[c + 1] = fmaf(x[c + 1], kc.y * factor, lv.y);
+                                x[c + 2] = fmaf(x[c + 2], kc.z * factor, lv.z);
+                                x[c + 3] = fmaf(x[c + 3], kc.w * factor, lv.w);
                             }
                         }
-                    }
-                    const float base = ref == -INFINITY ? 0.0f : ref;
-                    float part[4] = {};
+                        uint32_t seen[2] = {meta.there[2 * j], meta.there[2 * j + 1]};
+                        if ((seen[0] & seen[1]) != 0xffffffffu || !whole_strip(a, it, key0)) {
 #pragma unroll
-                    for (int c = 0; c < kTilesKeys; c += 32) {
-                        uint32_t w[16];
+                            for (int w = 0; w < 2; ++w) {
+                                uint32_t bits = first_bits(pos - key0 + 1, w);
+                                if (a.window > 0)
+                                    bits &= ~first_bits(pos - a.window - key0 + 1, w) | first_bits(a.sinks - key0, w);
+                                seen[w] &= bits;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float p0 = ex2(fmaf(x[c + i], scale, -base)), p1 = ex2(fmaf(x[c + i + 1], scale, -base));
-                            if constexpr (QUANT) {
-                                const float2 un = *reinterpret_cast<const float2*>(meta.unscale + c + i);
-                                part[i & 2] = fmaf(p0, un.x, part[i & 2]);
-                                part[(i & 2) + 1] = fmaf(p1, un.y, part[(i & 2) + 1]);
-                            } else {
-                                part[i & 2] += p0;
-                                part[(i & 2) + 1] += p1;
+                                for (int c = 0; c < 32; ++c)
+                                    x[w * 32 + c] = (seen[w] & (1u << c)) != 0 ? x[w * 32 + c] : -INFINITY;
                             }
-                            // the weights in the values' 16 bits; their sum above in fp32
-                            w[i / 2] = pack2<M>(p0, p1);
                         }
-                        tmem_store16(s_at + c / 2, w);
+                        float tops[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                        for (int c = 4; c < kStrip - 4; c += 8) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[c + i], x[c + 4 + i]);
+                        }
+                        float top = max3(max3(tops[0], x[60], x[61]), max3(tops[1], x[62], x[63]), fmaxf(tops[2], tops[3]));
+                        top *= scale;
+                        const bool grew = top > ref + (ref == -INFINITY ? 0.0f : kGrowth);
+                        if (__any_sync(0xffffffffu, grew)) {
+                            const float to = grew ? top : ref;
+                            const float alpha = grew ? ex2(ref - to) : 1.0f;
+                            ref = to;
+                            sum *= alpha;
+                            if (t > t0 || j > 0) {
+                                // the product of the strip before may still be adding to O
+                                ok = tile_wait(sm, &sm.o_done[h], (2 * ns + j - 1) & 1, polls);
+                                ok = __all_sync(0xffffffffu, ok);
+                                tmem_fence_after();
+#pragma unroll 1
+                                for (int c = 0; c < DPAD; c += 32) {
+                                    uint32_t o[32];
+                                    tmem_load32(o_at + c, o);
+                                    tmem_wait_load();
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                    tmem_store32(o_at + c, o);
+                                }
+                            }
+                        }
+                        const float base = ref == -INFINITY ? 0.0f : ref;
+                        const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
+                        float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                        for (int c = 0; c < kStrip; c += 32) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                float2 p = fma2(make_float2(x[c + i], x[c + i + 1]), scale2, base2);
+                                p = make_float2(ex2(p.x), ex2(p.y));
+                                if constexpr (QUANT)
+                                    part[i / 2 & 1] = fma2(
+                                        p, *reinterpret_cast<const float2*>(meta.unscale + j * kStrip + c + i), part[i / 2 & 1]);
+                                else
+                                    part[i / 2 & 1] = add2(part[i / 2 & 1], p);
+                                // the weights in the values' 16 bits; their sum above in fp32
+                                w[i / 2] = pack2<M>(p.x, p.y);
+                            }
+                            tmem_store16(strip + c / 2, w);
+                        }
+                        part[0] = add2(part[0], part[1]);
+                        sum += part[0].x + part[0].y;
+                        tmem_wait_store();
                     }
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
-                    tmem_wait_store();
+                    tmem_fence_before();
+                    mbar_arrive(&sm.p_full[h][j]);
                 }
-                tmem_fence_before();
-                mbar_arrive(&sm.p_full[h]);
             }
             // The next item's rows while this one's last product runs.
             const Item done = it;
@@ -600,51 +681,73 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
                 load_q();
                 loaded = true;
             }
-            ok = ok && tile_wait(sm, &sm.o_full[h], no & 1, polls);
+            ok = ok && tile_wait(sm, &sm.o_full[h], no++ & 1, polls);
             ok = __all_sync(0xffffffffu, ok);
-            ++no;
             tmem_fence_after();
             const bool begins = t0 == 0, ends = t_end == done.tiles;
-            const int r = h * 128 + row;
             if (rows) {
+                // 64 bytes of a row at a time go through shared memory, so that four lanes write them.
+                const int r = row0 + lane;
+                const bool real = r < done.rows;
                 Block* const block = reinterpret_cast<Block*>(a.partial) + 2 * blockIdx.x + (begins ? 1 : 0);
                 const float nan = __int_as_float(0x7fffffff);
                 const float inv = !ok ? nan : sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
-                T* const to = static_cast<T*>(a.out) +
-                              (r < done.rows ? row_offset(a, done, done.row0 + r, a.ob, a.os, a.oh) : 0);
-#pragma unroll
+                const int64_t mine = real ? row_offset(a, done, done.row0 + r, a.ob, a.os, a.oh) : -1;
+                auto put = [&](int i, const uint4& v) { staging[lane * 4 + (i ^ (lane >> 1 & 3))] = v; };
+                auto get = [&](int k) {
+                    const int to = k * 8 + lane / 4;
+                    return staging[to * 4 + (lane % 4 ^ (to >> 1 & 3))];
+                };
+#pragma unroll 1
                 for (int c = 0; c < DPAD; c += 32) {
                     uint32_t o[32];
-                    __syncwarp();
                     tmem_load32(o_at + c, o);
                     tmem_wait_load();
-                    if (r >= done.rows) {
-                        // a row of the tile that the item does not have
-                    } else if (begins && ends) {
+                    if (begins && ends) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            if (c + i >= a.cache.head_dim) break;
+                        for (int i = 0; i < 4; ++i) {
                             Packed<T, 8> y;
 #pragma unroll
                             for (int e = 0; e < 8; e += 2)
-                                put2(y, e, __uint_as_float(o[i + e]) * inv, __uint_as_float(o[i + e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(to + c + i) = *reinterpret_cast<uint4*>(&y);
+                                put2(y, e, __uint_as_float(o[i * 8 + e]) * inv, __uint_as_float(o[i * 8 + e + 1]) * inv);
+                            put(i, *reinterpret_cast<uint4*>(&y));
                         }
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int64_t to = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
+                            const int col = c + lane % 4 * 8;
+                            if (to >= 0 && col < a.cache.head_dim)
+                                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to + col) = get(k);
+                        }
+                        __syncwarp();
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4*>(&block->o[r][c + i]) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t* const w = o + half * 16 + i * 4;
+                                put(i, make_uint4(w[0], w[1], w[2], w[3]));
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int to = row0 + k * 8 + lane / 4;
+                                if (to < done.rows)
+                                    *reinterpret_cast<uint4*>(&block->o[to][c + half * 16 + lane % 4 * 4]) = get(k);
+                            }
+                            __syncwarp();
+                        }
                     }
                 }
-                if (r < done.rows) {
-                    if (!(begins && ends)) {
-                        block->m[r] = ref;
-                        block->l[r] = ok ? sum : nan;
-                    }
-                    if (sm.odd) {
-                        if (begins && ends) add_odd_values<T, QUANT, T>(a, done, t0, t_end, r, to);
-                        else add_odd_values<T, QUANT, float>(a, done, t0, t_end, r, block->o[r]);
-                    }
+                if (real && !(begins && ends)) {
+                    block->m[r] = ref;
+                    block->l[r] = ok ? sum : nan;
+                }
+                if (sm.odd) {
+                    __syncwarp();  // orders the row's stores by other lanes before this one's
+                    if (real && begins && ends) add_odd_values<T, QUANT, T>(a, done, t0, t_end, r, static_cast<T*>(a.out) + mine);
+                    else if (real) add_odd_values<T, QUANT, float>(a, done, t0, t_end, r, block->o[r]);
                 }
             }
             tmem_fence_before();
@@ -652,12 +755,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
                 a.joins[blockIdx.x] = make_int4(done.b, done.rt, done.h, owner(share, after + (done.tiles - t_end) - 1));
             if (!more) break;
         }
+        asm volatile("bar.arrive 2, 416;" ::: "memory");
     }
-    tmem_fence_before();
-    __syncthreads();
-    tmem_fence_after();
-    if (tid == 0 && sm.stop) *reinterpret_cast<volatile int*>(args.status) = kStatusWaitTimeout;
-    if (warp == 12) tmem_free<512>(tmem);
 }
 
 }  // namespace ako_b200
