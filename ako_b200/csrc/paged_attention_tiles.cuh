@@ -3,15 +3,20 @@
 //
 // A CTA holds 256 rows of one sequence and kv head (new tokens times the q
 // heads that share it) as two halves of 128 and goes over the keys in tiles of
-// 128, one CTA per SM. The scores S = Q K^T of a half and 64 keys go to tensor
-// memory; the half's four warps, a row to a thread, take them from there, write
-// the weights P over them in 16 bits, and O += P V reads P from tensor memory.
-// Each half has two such strips of 64 scores, so that its warps always have
-// one to work on while the tensor cores turn the other from P into the next S:
+// 128, one CTA per SM. The scores S = Q K^T of a half go to tensor memory; its
+// four warps, a row to a thread, take them from there, write the weights P over
+// them in 16 bits, and O += P V reads P from tensor memory, the first 96 keys'
+// (PV) as soon as they are there and the last 32 keys' (pv) with the next S.
+// While one half's warps work on their softmax the tensor cores work for the
+// other's:
 //
-//   tensor cores  | O_a += P_a0 V, S_a0 | O_b += P_b0 V, S_b0 | O_a += P_a1 V, S_a1 | ...
-//   half a's warps| softmax of S_a1 ...       | softmax of S_a0 ...
-//   half b's warps| softmax of S_b1 ...             | softmax of S_b0 ...
+//   tensor cores  | PV_a | pv_a, S_a | PV_b | pv_b, S_b | PV_a | pv_a, S_a | ...
+//   half a's warps| soft-|           | softmax of S_a          |
+//   half b's warps| softmax              |              | softmax of S_b ...
+//
+// S is taken 128 keys at a time because a product of 128 x 64 reads shared
+// memory for its first operand at more than the tensor cores' own rate (391
+// cycles measured against 260, and 520 for 128 x 128).
 //
 // Four more warps bring keys and values into shared memory (rows anywhere in
 // the cache, swizzled for the products), and one thread issues the products.
@@ -36,7 +41,7 @@ namespace ako_b200 {
 constexpr int kTilesThreads = 512;
 constexpr int kTilesRows = 256;
 constexpr int kTilesKeys = 128;
-constexpr int kStrip = 64;  // keys of a strip of scores
+constexpr int kEarly = 96;  // keys whose weights are handed on before the tile's others
 // Tiles whose key data are kept: the loading warps find a tile's keys one tile
 // before they bring them, at most STAGES + 2 tiles ahead of the softmax.
 constexpr int kMetaStages = 8;
@@ -70,7 +75,7 @@ template <int STAGES>
 struct TilesShared {
     TileMeta meta[kMetaStages];
     uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2], o_full[2], drained;
+    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drained;
     uint4 staging[8][128];  // of a softmax warp: 32 rows of 64 bytes on their way out
     uint32_t tmem;
     volatile int stop;     // a wait ran out
@@ -93,11 +98,6 @@ __device__ __forceinline__ bool tile_wait(S& sm, uint64_t* bar, uint32_t phase, 
 __device__ __forceinline__ bool whole_tile(const AttnArgs& a, const Item& it, int key0) {
     return key0 + kTilesKeys - 1 <= it.p_lo &&
            (a.window == 0 || key0 > it.p_hi - a.window || key0 + kTilesKeys <= a.sinks);
-}
-
-// The same for a strip.
-__device__ __forceinline__ bool whole_strip(const AttnArgs& a, const Item& it, int key0) {
-    return key0 + kStrip - 1 <= it.p_lo && (a.window == 0 || key0 > it.p_hi - a.window || key0 + kStrip <= a.sinks);
 }
 
 __device__ __forceinline__ bool sees_key(const AttnArgs& a, int pos, int key) {
@@ -218,13 +218,15 @@ struct TileLoader {
 
     // 16-bit caches: copies straight into the tile.
     __device__ __forceinline__ void copy(const void* base, int64_t offset, uint32_t tile) const {
+        // The places first: the copies' order is fixed, and each would wait for its own.
+        int64_t o[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) o[i] = __shfl_sync(0xffffffffu, offset, row0 + i * ROWS);
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int row = row0 + i * ROWS;
-            const int64_t o = __shfl_sync(0xffffffffu, offset, row);
-            const bool there = o >= 0 && real;
-            cp_async16_or_zero(tile + place(warp * 32 + row, chunk),
-                               there ? static_cast<const uint8_t*>(base) + (o + chunk * 8) * 2 : base, there);
+            const bool there = o[i] >= 0 && real;
+            cp_async16_or_zero(tile + place(warp * 32 + row0 + i * ROWS, chunk),
+                               static_cast<const uint8_t*>(base) + (there ? (o[i] + chunk * 8) * 2 : 0), there);
         }
     }
 
@@ -309,12 +311,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
         }
         for (int h = 0; h < 2; ++h) {
             mbar_init(&sm.q_full[h], 128);
-            mbar_init(&sm.o_done[h], 1);
+            mbar_init(&sm.s_full[h], 1);
+            mbar_init(&sm.p_full[h][0], 128);
+            mbar_init(&sm.p_full[h][1], 128);
             mbar_init(&sm.o_full[h], 1);
-            for (int j = 0; j < 2; ++j) {
-                mbar_init(&sm.s_full[h][j], 1);
-                mbar_init(&sm.p_full[h][j], 128);
-            }
         }
         mbar_init(&sm.drained, 1);
         fence_mbar_init();
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
         // elected lane issues the products and commits them.
         const bool leader = elect_one();
         const int steps = (a.cache.head_dim + 15) / 16;
-        const uint32_t s_shape = mma_shape(128, kStrip, TYPE, false);
+        const uint32_t s_shape = mma_shape(128, kTilesKeys, TYPE, false);
         const uint32_t o_shape = mma_shape(128, steps * 16, TYPE, true);
         constexpr uint32_t BLOCK = kTilesKeys * 128;  // bytes of 64 columns of a tile
         // a descriptor's address counts 16 bytes
@@ -359,49 +359,52 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
             ok = __all_sync(0xffffffffu, ok);
             return ok;
         };
-        // O_h (+)= P_h V of strip j of the half's tile `mine`, the CTA's tile `tile`
-        auto weigh = [&](int h, int j, uint32_t mine, uint32_t tile, bool add) {
-            if (!await(&sm.p_full[h][j], mine)) return;
-            if (j == 0 && h == 0) {
+        // O_h (+)= P_h V over the half's last tile of scores, the CTA's tile `tile`
+        auto weigh = [&](int h, uint32_t tile, bool add) {
+            const uint64_t v = v_desc + (tile % STAGES) * Shape::kOperand / 16;
+            const uint32_t o = tmem + O_COL + h * 128, p = tmem + h * 128;
+            if (h == 0) {
                 if (!await(&sm.v_full[tile % STAGES], tile / STAGES)) return;
-                fence_proxy_async_smem();  // the copies were not this proxy's
+                fence_proxy_async_smem();
             }
-            tmem_fence_after();
-            const uint64_t v = v_desc + ((tile % STAGES) * Shape::kOperand + j * kStrip * 128) / 16;
-            const uint32_t o = tmem + O_COL + h * 128, p = tmem + h * 128 + j * kStrip;
-            if (leader) {
 #pragma unroll
-                for (int k = 0; k < kStrip / 16; ++k) mma_ts(o, p + k * 8, v + k * (16 * 128 / 16), o_shape, add || k > 0);
-                mma_commit(&sm.o_done[h]);
+            for (int part = 0; part < 2; ++part) {
+                if (!await(&sm.p_full[h][part], ns[h] - 1)) return;
+                tmem_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < kTilesKeys / 16; ++k)
+                        if ((k < kEarly / 16) == (part == 0))
+                            mma_ts(o, p + k * 8, v + k * (16 * 128 / 16), o_shape, add || k > 0);
+                }
             }
         };
         do {
             const int t_end = part_end();
             const int halves = it.rows > 128 ? 2 : 1;
             for (int t = share.t; t < t_end && ok; ++t, ++n) {
+                if (t == share.t) {
+                    await(&sm.q_full[0], nq[0]++);
+                    if (halves == 2) await(&sm.q_full[1], nq[1]++);
+                }
                 await(&sm.k_full[n % STAGES], n / STAGES);
-                fence_proxy_async_smem();
+                fence_proxy_async_smem();  // the copies were not this proxy's
+                const uint64_t k = k_desc + (n % STAGES) * Shape::kOperand / 16;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h >= halves || !ok) break;
-                        if (t > share.t) weigh(h, j, ns[h] - 1, n - 1, j > 0 || t - 1 > share.t);
-                        else if (j == 0) await(&sm.q_full[h], nq[h]++);
-                        if (!ok) break;
-                        tmem_fence_after();
+                for (int h = 0; h < 2; ++h) {
+                    if (h >= halves || !ok) break;
+                    if (t > share.t) weigh(h, n - 1, t - 1 > share.t);
+                    if (!ok) break;
+                    if (leader) {
                         const uint64_t q = q_desc + h * Shape::kOperand / 16;
-                        const uint64_t k = k_desc + ((n % STAGES) * Shape::kOperand + j * kStrip * 128) / 16;
-                        if (leader) {
 #pragma unroll
-                            for (int s = 0; s < DPAD / 16; ++s) {
-                                const uint32_t to = ((s >> 2) * BLOCK + (s & 3) * 32) / 16;
-                                if (s < steps) mma_ss(tmem + h * 128 + j * kStrip, q + to, k + to, s_shape, s > 0);
-                            }
-                            mma_commit(&sm.s_full[h][j]);
+                        for (int s = 0; s < DPAD / 16; ++s) {
+                            const uint32_t to = ((s >> 2) * BLOCK + (s & 3) * 32) / 16;
+                            if (s < steps) mma_ss(tmem + h * 128, q + to, k + to, s_shape, s > 0);
                         }
-                        if (j == 1) ++ns[h];
+                        mma_commit(&sm.s_full[h]);
                     }
+                    ++ns[h];
                 }
                 if (leader) {
                     if (t > share.t) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
@@ -409,13 +412,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h >= halves || !ok) break;
-                    weigh(h, j, ns[h] - 1, n - 1, j > 0 || t_end - 1 > share.t);
-                    if (j == 1 && leader) mma_commit(&sm.o_full[h]);
-                }
+            for (int h = 0; h < 2; ++h) {
+                if (h >= halves || !ok) break;
+                weigh(h, n - 1, t_end - 1 > share.t);
+                if (leader) mma_commit(&sm.o_full[h]);
+            }
             if (leader) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
             if (!advance(t_end)) break;
         } while (ok);
@@ -523,6 +524,20 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
             const bool real = r < it.rows;
             pos = real ? it.kv - it.n + static_cast<int>(a.by_group.div(it.row0 + r)) : it.p_hi;
             const int64_t mine = real ? row_offset(a, it, it.row0 + r, a.qb, a.qs, a.qh) : -1;
+            if (!QUANT && args.q_factor == 1.0f) {  // as it is
+                int64_t o[TIMES];
+#pragma unroll
+                for (int i = 0; i < TIMES; ++i) o[i] = __shfl_sync(0xffffffffu, mine, i * TAKEN + lane / LANES);
+#pragma unroll
+                for (int i = 0; i < TIMES; ++i) {
+                    const bool there = o[i] >= 0 && c * 8 < a.cache.head_dim;
+                    cp_async16_or_zero(smem_addr(my_q) + TileLoader<T, QUANT, DPAD>::place(
+                                                             (warp & 3) * 32 + i * TAKEN + lane / LANES, c),
+                                       static_cast<const T*>(a.q) + (there ? o[i] + c * 8 : 0), there);
+                }
+                mbar_arrive_copied(&sm.q_full[h]);
+                return;
+            }
             factor = 1.0f;
             Packed<T, 8> x[TIMES];
 #pragma unroll
@@ -577,100 +592,100 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
             float ref = -INFINITY, sum = 0.0f;
             for (int t = t0; t < t_end && ok; ++t, ++n, ++ns) {
                 const TileMeta& meta = sm.meta[n % kMetaStages];
-#pragma unroll 1
-                for (int j = 0; j < 2; ++j) {
-                    const int key0 = key_tile(it, t) * kTilesKeys + j * kStrip;
-                    const uint32_t strip = s_at + j * kStrip;
-                    ok = tile_wait(sm, &sm.s_full[h][j], ns & 1, polls);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tmem_fence_after();
-                    if (rows) {
-                        float x[kStrip];
+                const int key0 = key_tile(it, t) * kTilesKeys;
+                ok = tile_wait(sm, &sm.s_full[h], ns & 1, polls);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tmem_fence_after();
+                if (rows) {
+                    float x[kTilesKeys];
 #pragma unroll
-                        for (int c = 0; c < kStrip; c += 32) tmem_load32(strip + c, reinterpret_cast<uint32_t*>(x + c));
-                        tmem_wait_load();
-                        if constexpr (QUANT) {
+                    for (int c = 0; c < kTilesKeys; c += 32) tmem_load32(s_at + c, reinterpret_cast<uint32_t*>(x + c));
+                    const uint4 there = *reinterpret_cast<const uint4*>(meta.there);
+                    const bool whole = (there.x & there.y & there.z & there.w) == 0xffffffffu && whole_tile(a, it, key0);
+                    tmem_wait_load();
+                    if constexpr (QUANT) {
 #pragma unroll
-                            for (int c = 0; c < kStrip; c += 4) {
-                                const float4 kc = *reinterpret_cast<const float4*>(meta.kc + j * kStrip + c);
-                                const float4 lv = *reinterpret_cast<const float4*>(meta.lv + j * kStrip + c);
-                                x[c] = fmaf(x[c], kc.x * factor, lv.x);
-                                x[c + 1] = fmaf(x[c + 1], kc.y * factor, lv.y);
-                                x[c + 2] = fmaf(x[c + 2], kc.z * factor, lv.z);
-                                x[c + 3] = fmaf(x[c + 3], kc.w * factor, lv.w);
-                            }
+                        for (int c = 0; c < kTilesKeys; c += 4) {
+                            const float4 kc = *reinterpret_cast<const float4*>(meta.kc + c);
+                            const float4 lv = *reinterpret_cast<const float4*>(meta.lv + c);
+                            x[c] = fmaf(x[c], kc.x * factor, lv.x);
+                            x[c + 1] = fmaf(x[c + 1], kc.y * factor, lv.y);
+                            x[c + 2] = fmaf(x[c + 2], kc.z * factor, lv.z);
+                            x[c + 3] = fmaf(x[c + 3], kc.w * factor, lv.w);
                         }
-                        uint32_t seen[2] = {meta.there[2 * j], meta.there[2 * j + 1]};
-                        if ((seen[0] & seen[1]) != 0xffffffffu || !whole_strip(a, it, key0)) {
-#pragma unroll
-                            for (int w = 0; w < 2; ++w) {
-                                uint32_t bits = first_bits(pos - key0 + 1, w);
-                                if (a.window > 0)
-                                    bits &= ~first_bits(pos - a.window - key0 + 1, w) | first_bits(a.sinks - key0, w);
-                                seen[w] &= bits;
-#pragma unroll
-                                for (int c = 0; c < 32; ++c)
-                                    x[w * 32 + c] = (seen[w] & (1u << c)) != 0 ? x[w * 32 + c] : -INFINITY;
-                            }
-                        }
-                        float tops[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                        for (int c = 4; c < kStrip - 4; c += 8) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[c + i], x[c + 4 + i]);
-                        }
-                        float top = max3(max3(tops[0], x[60], x[61]), max3(tops[1], x[62], x[63]), fmaxf(tops[2], tops[3]));
-                        top *= scale;
-                        const bool grew = top > ref + (ref == -INFINITY ? 0.0f : kGrowth);
-                        if (__any_sync(0xffffffffu, grew)) {
-                            const float to = grew ? top : ref;
-                            const float alpha = grew ? ex2(ref - to) : 1.0f;
-                            ref = to;
-                            sum *= alpha;
-                            if (t > t0 || j > 0) {
-                                // the product of the strip before may still be adding to O
-                                ok = tile_wait(sm, &sm.o_done[h], (2 * ns + j - 1) & 1, polls);
-                                ok = __all_sync(0xffffffffu, ok);
-                                tmem_fence_after();
-#pragma unroll 1
-                                for (int c = 0; c < DPAD; c += 32) {
-                                    uint32_t o[32];
-                                    tmem_load32(o_at + c, o);
-                                    tmem_wait_load();
-#pragma unroll
-                                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                                    tmem_store32(o_at + c, o);
-                                }
-                            }
-                        }
-                        const float base = ref == -INFINITY ? 0.0f : ref;
-                        const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
-                        float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-                        for (int c = 0; c < kStrip; c += 32) {
-                            uint32_t w[16];
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                float2 p = fma2(make_float2(x[c + i], x[c + i + 1]), scale2, base2);
-                                p = make_float2(ex2(p.x), ex2(p.y));
-                                if constexpr (QUANT)
-                                    part[i / 2 & 1] = fma2(
-                                        p, *reinterpret_cast<const float2*>(meta.unscale + j * kStrip + c + i), part[i / 2 & 1]);
-                                else
-                                    part[i / 2 & 1] = add2(part[i / 2 & 1], p);
-                                // the weights in the values' 16 bits; their sum above in fp32
-                                w[i / 2] = pack2<M>(p.x, p.y);
-                            }
-                            tmem_store16(strip + c / 2, w);
-                        }
-                        part[0] = add2(part[0], part[1]);
-                        sum += part[0].x + part[0].y;
-                        tmem_wait_store();
                     }
-                    tmem_fence_before();
-                    mbar_arrive(&sm.p_full[h][j]);
+                    if (!whole) {
+                        uint32_t seen[4] = {there.x, there.y, there.z, there.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t bits = first_bits(pos - key0 + 1, w);
+                            if (a.window > 0)
+                                bits &= ~first_bits(pos - a.window - key0 + 1, w) | first_bits(a.sinks - key0, w);
+                            seen[w] &= bits;
+#pragma unroll
+                            for (int c = 0; c < 32; ++c)
+                                x[w * 32 + c] = (seen[w] & (1u << c)) != 0 ? x[w * 32 + c] : -INFINITY;
+                        }
+                    }
+                    float tops[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int c = 4; c < kTilesKeys - 4; c += 8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[c + i], x[c + 4 + i]);
+                    }
+                    float top = max3(max3(tops[0], x[124], x[125]), max3(tops[1], x[126], x[127]), fmaxf(tops[2], tops[3]));
+                    top *= scale;
+                    const bool grew = top > ref + (ref == -INFINITY ? 0.0f : kGrowth);
+                    if (__any_sync(0xffffffffu, grew)) {
+                        const float to = grew ? top : ref;
+                        const float alpha = grew ? ex2(ref - to) : 1.0f;
+                        ref = to;
+                        sum *= alpha;
+                        if (t > t0) {  // the products of the tile before are done: this tile's scores came after them
+#pragma unroll 1
+                            for (int c = 0; c < DPAD; c += 16) {
+                                uint32_t o[16];
+                                tmem_load16(o_at + c, o);
+                                tmem_wait_load();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                tmem_store16(o_at + c, o);
+                            }
+                        }
+                    }
+                    const float base = ref == -INFINITY ? 0.0f : ref;
+                    const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
+                    float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                    for (int c = 0; c < kTilesKeys; c += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float2 p = fma2(make_float2(x[c + i], x[c + i + 1]), scale2, base2);
+                            p = make_float2(ex2(p.x), ex2(p.y));
+                            if constexpr (QUANT)
+                                part[i / 2 & 1] = fma2(p, *reinterpret_cast<const float2*>(meta.unscale + c + i), part[i / 2 & 1]);
+                            else
+                                part[i / 2 & 1] = add2(part[i / 2 & 1], p);
+                            // the weights in the values' 16 bits; their sum above in fp32
+                            w[i / 2] = pack2<M>(p.x, p.y);
+                        }
+                        tmem_store16(s_at + c / 2, w);
+                        if (c + 32 == kEarly) {
+                            tmem_wait_store();
+                            tmem_fence_before();
+                            mbar_arrive(&sm.p_full[h][0]);
+                        }
+                    }
+                    part[0] = add2(part[0], part[1]);
+                    sum += part[0].x + part[0].y;
+                    tmem_wait_store();
+                } else {
+                    mbar_arrive(&sm.p_full[h][0]);
                 }
+                tmem_fence_before();
+                mbar_arrive(&sm.p_full[h][1]);
             }
             // The next item's rows while this one's last product runs.
             const Item done = it;
@@ -698,12 +713,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
                     const int to = k * 8 + lane / 4;
                     return staging[to * 4 + (lane % 4 ^ (to >> 1 & 3))];
                 };
-#pragma unroll 1
-                for (int c = 0; c < DPAD; c += 32) {
-                    uint32_t o[32];
-                    tmem_load32(o_at + c, o);
-                    tmem_wait_load();
-                    if (begins && ends) {
+                uint32_t all[DPAD];
+#pragma unroll
+                for (int c = 0; c < DPAD; c += 32) tmem_load32(o_at + c, all + c);
+                tmem_wait_load();
+                if (begins && ends) {
+                    int64_t to[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
+#pragma unroll
+                    for (int c = 0; c < DPAD; c += 32) {
+                        const uint32_t* const o = all + c;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             Packed<T, 8> y;
@@ -713,31 +733,27 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
                             put(i, *reinterpret_cast<uint4*>(&y));
                         }
                         __syncwarp();
+                        const int col = c + lane % 4 * 8;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (to[k] >= 0 && col < a.cache.head_dim)
+                                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to[k] + col) = get(k);
+                        __syncwarp();
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < DPAD; c += 16) {
+                        const uint32_t* const o = all + c;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) put(i, make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]));
+                        __syncwarp();
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const int64_t to = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
-                            const int col = c + lane % 4 * 8;
-                            if (to >= 0 && col < a.cache.head_dim)
-                                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to + col) = get(k);
+                            const int to = row0 + k * 8 + lane / 4;
+                            if (to < done.rows)
+                                *reinterpret_cast<uint4*>(&block->o[to][c + lane % 4 * 4]) = get(k);
                         }
                         __syncwarp();
-                    } else {
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t* const w = o + half * 16 + i * 4;
-                                put(i, make_uint4(w[0], w[1], w[2], w[3]));
-                            }
-                            __syncwarp();
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const int to = row0 + k * 8 + lane / 4;
-                                if (to < done.rows)
-                                    *reinterpret_cast<uint4*>(&block->o[to][c + half * 16 + lane % 4 * 4]) = get(k);
-                            }
-                            __syncwarp();
-                        }
                     }
                 }
                 if (real && !(begins && ends)) {
