@@ -52,6 +52,10 @@ constexpr int kSoftmaxRegs = 184, kLoadRegs = 96, kIssueRegs = 48;
 constexpr float kGrowth = 8.0f;  // log2 of the factor by which a maximum may lag
 
 struct TilesArgs {
+    // The cache's keys and values as (page, head, slot, column) in boxes of `box` slots and 64
+    // columns, swizzled as the tiles are; box is 0 where pages do not divide into such boxes.
+    CUtensorMap k_map, v_map;
+    int box;
     AttnArgs a;
     int* status;
     uint32_t wait_polls;
@@ -149,8 +153,12 @@ __device__ __forceinline__ bool scrub(uint4& v) {
     return any != 0;
 }
 
-// One of the four loading warps, which brings 32 keys of every tile. A lane
-// looks after one key's place in the cache and copies chunks of several rows.
+// One of the four loading warps. In an e4m3 cache each brings 32 keys of every
+// tile and their values; in a 16-bit cache, whose copies need no registers,
+// two warps bring 64 keys each and two 64 values each, so that neither waits
+// for the other's stage. A lane looks after one place in the cache (or two)
+// and copies chunks of several rows; 64 rows of which every row of q sees every
+// key come as boxes of a tensor map instead, where the pages allow it.
 template <typename T, bool QUANT, int DPAD>
 struct TileLoader {
     static constexpr int ES = QUANT ? 1 : 2;
@@ -158,7 +166,7 @@ struct TileLoader {
     static constexpr int ROWS = 32 / CHUNKS;       // rows that the warp takes at once
     static constexpr int EACH = 32 / ROWS;         // chunks of a lane
     const AttnArgs& a;
-    int warp, lane, chunk, row0;
+    int rows0, lane, chunk, row0;  // the warp's first row of a tile; the lane's among those taken at once
     bool real;  // the chunk lies within head_dim
 
     // A key's place, as far as it is known: its table entry is on the way.
@@ -173,17 +181,18 @@ struct TileLoader {
         bool whole;
     };
 
-    __device__ TileLoader(const AttnArgs& args, int w, int l)
-        : a(args), warp(w), lane(l), chunk(l % CHUNKS), row0(l / CHUNKS), real(chunk * 16 < args.cache.head_dim * ES) {}
+    __device__ TileLoader(const AttnArgs& args, int first, int l)
+        : a(args), rows0(first), lane(l), chunk(l % CHUNKS), row0(l / CHUNKS), real(chunk * 16 < args.cache.head_dim * ES) {}
 
     // Where the 16-bit chunk c of a row goes in a tile.
     static __device__ __forceinline__ uint32_t place(int row, int c) {
         return static_cast<uint32_t>((c >> 3) * (kTilesKeys * 128) + row * 128 + ((c & 7) ^ (row & 7)) * 16);
     }
 
-    __device__ __forceinline__ Place look_up(const Item& it, int key0) const {
+    // Of the lane's key, `more` rows behind its first.
+    __device__ __forceinline__ Place look_up(const Item& it, int key0, int more = 0) const {
         Place p{-1, 0, it.h, whole_tile(a, it, key0)};
-        const int key = key0 + warp * 32 + lane;
+        const int key = key0 + rows0 + more + lane;
         if (key <= it.p_hi && (key >= it.win_lo || key < a.sinks)) {
             const int i = static_cast<int>(a.cache.by_page.div(static_cast<uint32_t>(key)));
             p.slot = key - i * a.cache.page_size;
@@ -192,10 +201,17 @@ struct TileLoader {
         return p;
     }
 
-    __device__ __forceinline__ Rows find(const Place& p, TileMeta& meta) const {
+    __device__ __forceinline__ bool there(const Place& p) const { return p.page >= 0 && p.page < a.cache.num_pages; }
+
+    // Notes which of 32 keys, `more` rows behind the warp's first, are there.
+    __device__ __forceinline__ void put_there(const Place& p, TileMeta& meta, int more = 0) const {
+        const unsigned bits = __ballot_sync(0xffffffffu, there(p));
+        if (lane == 0) meta.there[(rows0 + more) / 32] = bits;
+    }
+
+    __device__ __forceinline__ Rows find(const Place& p) const {
         Rows r{-1, -1, 0.0f, 1.0f, p.whole};
-        const bool there = p.page >= 0 && p.page < a.cache.num_pages;
-        if (there) {
+        if (there(p)) {
             r.k = a.cache.k.offset(p.page, p.h, p.slot);
             r.v = a.cache.v.offset(p.page, p.h, p.slot);
             if constexpr (QUANT) {
@@ -203,21 +219,20 @@ struct TileLoader {
                 r.vs = static_cast<const float*>(a.cache.vs.p)[a.cache.vs.offset(p.page, p.h, p.slot)];
             }
         }
-        const unsigned bits = __ballot_sync(0xffffffffu, there);
-        if (lane == 0) meta.there[warp] = bits;
         return r;
     }
 
     // An e4m3 cache's scales, as the kernel for few rows has them.
     __device__ __forceinline__ void put_scales(const Rows& r, TileMeta& meta) const {
         const float vs = fmaxf(r.vs, 0x1p-100f);
-        meta.kc[warp * 32 + lane] = r.ks * a.scale;
-        meta.lv[warp * 32 + lane] = __log2f(vs);
-        meta.unscale[warp * 32 + lane] = __fdividef(1.0f, vs);
+        meta.kc[rows0 + lane] = r.ks * a.scale;
+        meta.lv[rows0 + lane] = __log2f(vs);
+        meta.unscale[rows0 + lane] = __fdividef(1.0f, vs);
     }
 
     // 16-bit caches: copies straight into the tile.
-    __device__ __forceinline__ void copy(const void* base, int64_t offset, uint32_t tile) const {
+    __device__ __forceinline__ void copy(const PagedTensor& from, const Place& p, uint32_t tile, int more) const {
+        const int64_t offset = there(p) ? from.offset(p.page, p.h, p.slot) : -1;
         // The places first: the copies' order is fixed, and each would wait for its own.
         int64_t o[EACH];
 #pragma unroll
@@ -225,8 +240,8 @@ struct TileLoader {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const bool there = o[i] >= 0 && real;
-            cp_async16_or_zero(tile + place(warp * 32 + row0 + i * ROWS, chunk),
-                               static_cast<const uint8_t*>(base) + (there ? (o[i] + chunk * 8) * 2 : 0), there);
+            cp_async16_or_zero(tile + place(rows0 + more + row0 + i * ROWS, chunk),
+                               static_cast<const uint8_t*>(from.p) + (there ? (o[i] + chunk * 8) * 2 : 0), there);
         }
     }
 
@@ -234,8 +249,8 @@ struct TileLoader {
     __device__ __forceinline__ bool scrub_copied(uint8_t* tile) const {
         bool any = false;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            uint4* const p = reinterpret_cast<uint4*>(tile + place(warp * 32 + row0 + i * ROWS, chunk));
+        for (int i = 0; i < 2 * EACH; ++i) {
+            uint4* const p = reinterpret_cast<uint4*>(tile + place(rows0 + row0 + i * ROWS, chunk));
             uint4 v = *p;
             if (scrub<T>(v)) {
                 *p = v;
@@ -266,7 +281,7 @@ struct TileLoader {
                 uint4 w = make_uint4(e4m3x2_to_half2(u[2 * half]), e4m3x2_to_half2(u[2 * half] >> 16),
                                      e4m3x2_to_half2(u[2 * half + 1]), e4m3x2_to_half2(u[2 * half + 1] >> 16));
                 if (clean && scrub<__half>(w)) any = true;
-                *reinterpret_cast<uint4*>(tile + place(warp * 32 + row0 + i * ROWS, chunk * 2 + half)) = w;
+                *reinterpret_cast<uint4*>(tile + place(rows0 + row0 + i * ROWS, chunk * 2 + half)) = w;
             }
         }
         return any;
@@ -280,7 +295,7 @@ __device__ __forceinline__ uint32_t first_bits(int n, int w) {
 }
 
 template <typename T, bool QUANT, int DPAD>
-__global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const TilesArgs args) {
+__global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __grid_constant__ TilesArgs args) {
     pdl_enter();
     using Shape = TilesShape<DPAD>;
     using M = std::conditional_t<QUANT, __half, T>;
@@ -304,8 +319,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
     if (!find_share<kTilesRows, kTilesKeys, kTilesThreads>(a, 1, sm.scratch, share)) return;
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&sm.k_full[i], 128);
-            mbar_init(&sm.v_full[i], 128);
+            mbar_init(&sm.k_full[i], QUANT ? 128 : 64);
+            mbar_init(&sm.v_full[i], QUANT ? 128 : 64);
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
         }
@@ -433,74 +448,108 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const Tile
         // ----------------------------------------------------------- loading
         give_registers<kLoadRegs>();
         using Loader = TileLoader<T, QUANT, DPAD>;
-        const Loader load(a, warp & 3, lane);
-        const uint32_t k_addr = smem_addr(k_tile), v_addr = smem_addr(v_tile);
+        const Loader load(a, QUANT ? (warp & 3) * 32 : (warp & 1) * 64, lane);
         bool ok = true;
         auto acquire = [&](uint64_t* empty, uint32_t use) {
             ok = ok && tile_wait(sm, empty, ((use / STAGES) & 1) ^ 1, polls);
             ok = __all_sync(0xffffffffu, ok);
         };
-        // The table entries of a tile's keys are asked for two tiles ahead and its rows known one
-        // tile ahead, so that a tile waits for neither.
+        // The table entries of a tile's keys are asked for ahead of the tile (by two tiles in an
+        // e4m3 cache, whose scales are asked for by one), so that it does not wait for them.
         int t_end = part_end();
         int t = share.t;
-        bool last = false;  // nothing behind the tile looked up last
-        auto ahead = [&] {
-            if (++t == t_end) {
-                last = !advance(t_end);
-                t = 0;
-                t_end = last ? 1 : part_end();
-            }
-            return last ? typename Loader::Place{-1, 0, 0, true} : load.look_up(it, key_tile(it, t) * kTilesKeys);
+        // moves on to the next tile; false behind the last
+        auto step = [&] {
+            if (++t < t_end) return true;
+            if (!advance(t_end)) return false;
+            t = 0;
+            t_end = part_end();
+            return true;
         };
-        typename Loader::Rows rows = load.find(load.look_up(it, key_tile(it, t) * kTilesKeys), sm.meta[0]);
-        typename Loader::Place place = ahead();
-        bool more = !last;
-        [[maybe_unused]] uint4 kv[Loader::EACH], vv[Loader::EACH];
-        if constexpr (QUANT) {
+        auto key0 = [&] { return key_tile(it, t) * kTilesKeys; };
+        if constexpr (!QUANT) {
+            using Place = typename Loader::Place;
+            const bool values = (warp & 2) != 0;
+            const PagedTensor& from = values ? a.cache.v : a.cache.k;
+            uint8_t* const tile = values ? v_tile : k_tile;
+            const uint32_t tile_addr = smem_addr(tile);
+            uint64_t* const full = values ? sm.v_full : sm.k_full;
+            uint64_t* const empty = values ? sm.v_empty : sm.k_empty;
+            Place p0 = load.look_up(it, key0()), p1 = load.look_up(it, key0(), 32);
+            bool more = true;
+            for (uint32_t n = 0; more; ++n) {
+                const int st = n % STAGES;
+                const Place now0 = p0, now1 = p1;
+                more = step();
+                if (more) {
+                    p0 = load.look_up(it, key0());
+                    p1 = load.look_up(it, key0(), 32);
+                }
+                acquire(&empty[st], n);
+                if (!ok) break;
+                if (!values) {
+                    load.put_there(now0, sm.meta[n % kMetaStages]);
+                    load.put_there(now1, sm.meta[n % kMetaStages], 32);
+                }
+                if (args.box != 0 && now0.whole && __all_sync(0xffffffffu, load.there(now0) && load.there(now1))) {
+                    // Boxes of whole pages, or of 64 rows of one, a lane to each.
+                    constexpr int BLOCKS = DPAD / 64;
+                    const int r = lane / BLOCKS * args.box, block = lane % BLOCKS;
+                    const int page0 = __shfl_sync(0xffffffffu, now0.page, r & 31), page1 = __shfl_sync(0xffffffffu, now1.page, r & 31);
+                    const int slot0 = __shfl_sync(0xffffffffu, now0.slot, r & 31), slot1 = __shfl_sync(0xffffffffu, now1.slot, r & 31);
+                    if (lane == 0) mbar_expect_tx(&full[st], 64 * DPAD * 2);
+                    else mbar_arrive(&full[st]);
+                    __syncwarp();
+                    if (r < 64)
+                        tensor_load(tile_addr + st * Shape::kOperand + block * (kTilesKeys * 128) + ((warp & 1) * 64 + r) * 128,
+                                    values ? &args.v_map : &args.k_map, block * 64, r < 32 ? slot0 : slot1, now0.h,
+                                    r < 32 ? page0 : page1, &full[st]);
+                    continue;
+                }
+                load.copy(from, now0, tile_addr + st * Shape::kOperand, 0);
+                load.copy(from, now1, tile_addr + st * Shape::kOperand, 32);
+                if (!values || now0.whole) {
+                    mbar_arrive_copied(&full[st]);
+                } else {
+                    cp_async_wait_everything();
+                    if (load.scrub_copied(tile + st * Shape::kOperand)) sm.odd = 1;
+                    mbar_arrive(&full[st]);
+                }
+            }
+        } else {
+            typename Loader::Place place = load.look_up(it, key0());
+            load.put_there(place, sm.meta[0]);
+            typename Loader::Rows rows = load.find(place);
+            bool more = step();
+            if (more) place = load.look_up(it, key0());
+            uint4 kv[Loader::EACH], vv[Loader::EACH];
             load.fetch(a.cache.k.p, rows.k, kv);
             load.fetch(a.cache.v.p, rows.v, vv);
-        }
-        for (uint32_t n = 0;; ++n) {
-            const int st = n % STAGES;
-            const typename Loader::Rows now = rows;
-            uint8_t* const vt = v_tile + st * Shape::kOperand;
-            const bool next = more;
-            acquire(&sm.k_empty[st], n);
-            if (!ok) break;
-            if constexpr (QUANT) {
+            for (uint32_t n = 0;; ++n) {
+                const int st = n % STAGES;
+                const typename Loader::Rows now = rows;
+                const bool next = more;
+                acquire(&sm.k_empty[st], n);
+                if (!ok) break;
                 load.put_scales(now, sm.meta[n % kMetaStages]);
                 load.convert(kv, k_tile + st * Shape::kOperand, false);
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.k_full[st]);
-            } else {
-                load.copy(a.cache.k.p, now.k, k_addr + st * Shape::kOperand);
-                mbar_arrive_copied(&sm.k_full[st]);
-            }
-            if (next) {
-                rows = load.find(place, sm.meta[(n + 1) % kMetaStages]);
-                if constexpr (QUANT) load.fetch(a.cache.k.p, rows.k, kv);
-                place = ahead();
-                more = !last;
-            }
-            acquire(&sm.v_empty[st], n);
-            if (!ok) break;
-            if constexpr (QUANT) {
-                if (load.convert(vv, vt, !now.whole)) sm.odd = 1;
+                if (next) {
+                    load.put_there(place, sm.meta[(n + 1) % kMetaStages]);
+                    rows = load.find(place);
+                    load.fetch(a.cache.k.p, rows.k, kv);
+                    more = step();
+                    if (more) place = load.look_up(it, key0());
+                }
+                acquire(&sm.v_empty[st], n);
+                if (!ok) break;
+                if (load.convert(vv, v_tile + st * Shape::kOperand, !now.whole)) sm.odd = 1;
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.v_full[st]);
-                if (next) load.fetch(a.cache.v.p, rows.v, vv);
-            } else {
-                load.copy(a.cache.v.p, now.v, v_addr + st * Shape::kOperand);
-                if (now.whole) {
-                    mbar_arrive_copied(&sm.v_full[st]);
-                } else {
-                    cp_async_wait_everything();
-                    if (load.scrub_copied(vt)) sm.odd = 1;
-                    mbar_arrive(&sm.v_full[st]);
-                }
+                if (!next) break;
+                load.fetch(a.cache.v.p, rows.v, vv);
             }
-            if (!next) break;
         }
         cp_async_wait_everything();
         asm volatile("bar.arrive 2, 416;" ::: "memory");

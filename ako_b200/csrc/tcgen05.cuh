@@ -2,6 +2,8 @@
 // CTA per tile (cta_group::1), 16-bit operands and fp32 sums.
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace ako_b200 {
@@ -111,6 +113,16 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t one;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
     return one != 0;
+}
+
+// Copies the box of a 4-D tensor that starts at (x, y, z, w) to shared memory;
+// its bytes count on `bar`. x * element size is a multiple of 16. One thread.
+__device__ __forceinline__ void tensor_load(uint32_t to, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(to),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+        : "memory");
 }
 
 // Arrives on `bar` when this thread's cp.async copies so far have landed; the
