@@ -45,7 +45,8 @@ constexpr int kEarly = 96;  // keys whose weights are handed on before the tile'
 // Tiles whose key data are kept: the loading warps find a tile's keys one tile
 // before they bring them, at most STAGES + 2 tiles ahead of the softmax.
 constexpr int kMetaStages = 8;
-constexpr uint32_t kDrainLimit = 1u << 24;
+constexpr uint32_t kWaitCycles = 1u << 31;  // of a wait, about a second
+constexpr uint32_t kDrainPolls = 1u << 24;
 // Registers per thread of the softmax, loading and issuing warps. The block is
 // launched with 128 a thread, and 2 * 184 + 96 + 48 = 4 * 128.
 constexpr int kSoftmaxRegs = 184, kLoadRegs = 96, kIssueRegs = 48;
@@ -87,13 +88,21 @@ struct TilesShared {
     ShareScratch scratch;
 };
 
-// Waits for a phase of `bar`; false when the limit ran out, here or in another role.
-template <typename S>
-__device__ __forceinline__ bool tile_wait(S& sm, uint64_t* bar, uint32_t phase, uint32_t polls) {
+// Waits for a phase of `bar`, at most `polls` polls and a second or so (a poll
+// may sleep).
+__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t phase, uint32_t polls, const volatile int* stop) {
+    const uint32_t begin = static_cast<uint32_t>(clock());
     for (uint32_t i = 0; i < polls; ++i) {
         if (mbar_try_wait(bar, phase)) return true;
-        if (sm.stop) return false;
+        if (*stop || static_cast<uint32_t>(clock()) - begin > kWaitCycles) break;
     }
+    return false;
+}
+
+// The same for a role: when its limit runs out, all roles stop.
+template <typename S>
+__device__ __forceinline__ bool tile_wait(S& sm, uint64_t* bar, uint32_t phase, uint32_t polls) {
+    if (wait_bounded(bar, phase, polls, &sm.stop)) return true;
     sm.stop = 1;
     return false;
 }
@@ -357,7 +366,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         if (warp != 12) return;
         // The whole warp follows the loop, so that addresses and descriptors are uniform; one
         // elected lane issues the products and commits them.
-        const bool leader = elect_one();
         const int steps = (a.cache.head_dim + 15) / 16;
         const uint32_t s_shape = mma_shape(128, kTilesKeys, TYPE, false);
         const uint32_t o_shape = mma_shape(128, steps * 16, TYPE, true);
@@ -374,19 +382,24 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             ok = __all_sync(0xffffffffu, ok);
             return ok;
         };
+        // cp.async is not the products' proxy; tensor-map copies are.
+        auto order_copies = [&](bool whole) {
+            if (!QUANT && !(whole && args.box != 0)) fence_proxy_async_smem();
+        };
+        bool before = false;  // whether every row sees every key of the tile before
         // O_h (+)= P_h V over the half's last tile of scores, the CTA's tile `tile`
         auto weigh = [&](int h, uint32_t tile, bool add) {
             const uint64_t v = v_desc + (tile % STAGES) * Shape::kOperand / 16;
             const uint32_t o = tmem + O_COL + h * 128, p = tmem + h * 128;
             if (h == 0) {
                 if (!await(&sm.v_full[tile % STAGES], tile / STAGES)) return;
-                fence_proxy_async_smem();
+                order_copies(before);
             }
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
                 if (!await(&sm.p_full[h][part], ns[h] - 1)) return;
                 tmem_fence_after();
-                if (leader) {
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kTilesKeys / 16; ++k)
                         if ((k < kEarly / 16) == (part == 0))
@@ -403,14 +416,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                     if (halves == 2) await(&sm.q_full[1], nq[1]++);
                 }
                 await(&sm.k_full[n % STAGES], n / STAGES);
-                fence_proxy_async_smem();  // the copies were not this proxy's
+                const bool whole = whole_tile(a, it, key_tile(it, t) * kTilesKeys);
+                order_copies(whole && t > share.t);  // q is copied too
                 const uint64_t k = k_desc + (n % STAGES) * Shape::kOperand / 16;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (h >= halves || !ok) break;
                     if (t > share.t) weigh(h, n - 1, t - 1 > share.t);
                     if (!ok) break;
-                    if (leader) {
+                    if (elect_one()) {
                         const uint64_t q = q_desc + h * Shape::kOperand / 16;
 #pragma unroll
                         for (int s = 0; s < DPAD / 16; ++s) {
@@ -421,23 +435,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                     }
                     ++ns[h];
                 }
-                if (leader) {
+                if (elect_one()) {
                     if (t > share.t) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
                     mma_commit(&sm.k_empty[n % STAGES]);
                 }
+                before = whole;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (h >= halves || !ok) break;
                 weigh(h, n - 1, t_end - 1 > share.t);
-                if (leader) mma_commit(&sm.o_full[h]);
+                if (elect_one()) mma_commit(&sm.o_full[h]);
             }
-            if (leader) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
+            if (elect_one()) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
             if (!advance(t_end)) break;
         } while (ok);
         // nothing of this CTA's is under way when it gives its tensor memory back
-        if (leader) mma_commit(&sm.drained);
-        mbar_wait_bounded(&sm.drained, 0, kDrainLimit);
+        if (elect_one()) mma_commit(&sm.drained);
+        const volatile int never = 0;
+        wait_bounded(&sm.drained, 0, kDrainPolls, &never);
         __syncwarp();
         // the other roles are done with tensor memory
         asm volatile("bar.sync 2, 416;" ::: "memory");
@@ -508,11 +524,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 }
                 load.copy(from, now0, tile_addr + st * Shape::kOperand, 0);
                 load.copy(from, now1, tile_addr + st * Shape::kOperand, 32);
-                if (!values || now0.whole) {
+                if (now0.whole ? args.box == 0 : !values) {
                     mbar_arrive_copied(&full[st]);
                 } else {
                     cp_async_wait_everything();
-                    if (load.scrub_copied(tile + st * Shape::kOperand)) sm.odd = 1;
+                    if (!now0.whole && load.scrub_copied(tile + st * Shape::kOperand)) sm.odd = 1;
+                    fence_proxy_async_smem();
                     mbar_arrive(&full[st]);
                 }
             }
@@ -567,7 +584,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         float factor = 1.0f;
         // Brings the warp's rows of q into the half's tile, a row by DPAD / 8 lanes; `factor` takes
         // out what this thread's row was scaled by.
-        auto load_q = [&] {
+        auto load_q = [&](const Item& it) {
             constexpr int LANES = DPAD / 8, TAKEN = 32 / LANES, TIMES = 32 / TAKEN;
             const int r = row0 + lane, c = lane % LANES;
             const bool real = r < it.rows;
@@ -634,9 +651,26 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 if (!advance(t_end)) break;
                 continue;
             }
-            if (!loaded) load_q();
+            if (!loaded) load_q(it);
             // Warps without a row take part in the barriers alone.
             const bool rows = row0 < it.rows;
+            const int my_pos = pos;
+            const float my_factor = factor;
+            // The next item and its rows of q, which take the place of this one's once the last scores
+            // are there.
+            Item following;
+            bool more = false;
+            int64_t next_at = at;
+            loaded = false;
+            auto prepare_next = [&] {
+                next_at = at + (t_end - t0);
+                following = it;
+                more = next_at < share.end && next_item<kTilesRows, kTilesKeys>(a, following);
+                if (more && following.rows > h * 128) {
+                    load_q(following);
+                    loaded = true;
+                }
+            };
             const float scale = QUANT ? 1.0f : a.scale;
             float ref = -INFINITY, sum = 0.0f;
             for (int t = t0; t < t_end && ok; ++t, ++n, ++ns) {
@@ -646,6 +680,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tmem_fence_after();
+                if (t == t_end - 1) prepare_next();
                 if (rows) {
                     float x[kTilesKeys];
 #pragma unroll
@@ -658,23 +693,24 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                         for (int c = 0; c < kTilesKeys; c += 4) {
                             const float4 kc = *reinterpret_cast<const float4*>(meta.kc + c);
                             const float4 lv = *reinterpret_cast<const float4*>(meta.lv + c);
-                            x[c] = fmaf(x[c], kc.x * factor, lv.x);
-                            x[c + 1] = fmaf(x[c + 1], kc.y * factor, lv.y);
-                            x[c + 2] = fmaf(x[c + 2], kc.z * factor, lv.z);
-                            x[c + 3] = fmaf(x[c + 3], kc.w * factor, lv.w);
+                            x[c] = fmaf(x[c], kc.x * my_factor, lv.x);
+                            x[c + 1] = fmaf(x[c + 1], kc.y * my_factor, lv.y);
+                            x[c + 2] = fmaf(x[c + 2], kc.z * my_factor, lv.z);
+                            x[c + 3] = fmaf(x[c + 3], kc.w * my_factor, lv.w);
                         }
                     }
                     if (!whole) {
-                        uint32_t seen[4] = {there.x, there.y, there.z, there.w};
+                        const uint32_t seen[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            uint32_t bits = first_bits(pos - key0 + 1, w);
+                            uint32_t bits = first_bits(my_pos - key0 + 1, w);
                             if (a.window > 0)
-                                bits &= ~first_bits(pos - a.window - key0 + 1, w) | first_bits(a.sinks - key0, w);
-                            seen[w] &= bits;
+                                bits &= ~first_bits(my_pos - a.window - key0 + 1, w) | first_bits(a.sinks - key0, w);
+                            bits &= seen[w];
+                            if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
 #pragma unroll
                             for (int c = 0; c < 32; ++c)
-                                x[w * 32 + c] = (seen[w] & (1u << c)) != 0 ? x[w * 32 + c] : -INFINITY;
+                                x[w * 32 + c] = (bits & (1u << c)) != 0 ? x[w * 32 + c] : -INFINITY;
                         }
                     }
                     float tops[4] = {x[0], x[1], x[2], x[3]};
@@ -736,73 +772,72 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 tmem_fence_before();
                 mbar_arrive(&sm.p_full[h][1]);
             }
-            // The next item's rows while this one's last product runs.
-            const Item done = it;
-            const int64_t after = at + (t_end - t0);
-            const bool more = advance(t_end);
-            loaded = false;
-            if (more && it.rows > h * 128 && ok) {
-                load_q();
-                loaded = true;
+            if (!ok) {
+                loaded = false;
+                next_at = at + (t_end - t0);
+                following = it;
+                more = next_at < share.end && next_item<kTilesRows, kTilesKeys>(a, following);
             }
             ok = ok && tile_wait(sm, &sm.o_full[h], no++ & 1, polls);
             ok = __all_sync(0xffffffffu, ok);
             tmem_fence_after();
-            const bool begins = t0 == 0, ends = t_end == done.tiles;
+            const bool begins = t0 == 0, ends = t_end == it.tiles;
             if (rows) {
                 // 64 bytes of a row at a time go through shared memory, so that four lanes write them.
                 const int r = row0 + lane;
-                const bool real = r < done.rows;
+                const bool real = r < it.rows;
                 Block* const block = reinterpret_cast<Block*>(a.partial) + 2 * blockIdx.x + (begins ? 1 : 0);
                 const float nan = __int_as_float(0x7fffffff);
                 const float inv = !ok ? nan : sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
-                const int64_t mine = real ? row_offset(a, done, done.row0 + r, a.ob, a.os, a.oh) : -1;
+                const int64_t mine = real ? row_offset(a, it, it.row0 + r, a.ob, a.os, a.oh) : -1;
                 auto put = [&](int i, const uint4& v) { staging[lane * 4 + (i ^ (lane >> 1 & 3))] = v; };
                 auto get = [&](int k) {
                     const int to = k * 8 + lane / 4;
                     return staging[to * 4 + (lane % 4 ^ (to >> 1 & 3))];
                 };
-                uint32_t all[DPAD];
+                int64_t to[4];
 #pragma unroll
-                for (int c = 0; c < DPAD; c += 32) tmem_load32(o_at + c, all + c);
-                tmem_wait_load();
-                if (begins && ends) {
-                    int64_t to[4];
+                for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
+#pragma unroll 1
+                for (int c0 = 0; c0 < DPAD; c0 += 64) {
+                    uint32_t o[64];
+                    tmem_load32(o_at + c0, o);
+                    tmem_load32(o_at + c0 + 32, o + 32);
+                    tmem_wait_load();
+                    if (begins && ends) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
+                        for (int c = 0; c < 64; c += 32) {
 #pragma unroll
-                    for (int c = 0; c < DPAD; c += 32) {
-                        const uint32_t* const o = all + c;
+                            for (int i = 0; i < 4; ++i) {
+                                Packed<T, 8> y;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            Packed<T, 8> y;
+                                for (int e = 0; e < 8; e += 2)
+                                    put2(y, e, __uint_as_float(o[c + i * 8 + e]) * inv,
+                                         __uint_as_float(o[c + i * 8 + e + 1]) * inv);
+                                put(i, *reinterpret_cast<uint4*>(&y));
+                            }
+                            __syncwarp();
+                            const int col = c0 + c + lane % 4 * 8;
 #pragma unroll
-                            for (int e = 0; e < 8; e += 2)
-                                put2(y, e, __uint_as_float(o[i * 8 + e]) * inv, __uint_as_float(o[i * 8 + e + 1]) * inv);
-                            put(i, *reinterpret_cast<uint4*>(&y));
+                            for (int k = 0; k < 4; ++k)
+                                if (to[k] >= 0 && col < a.cache.head_dim)
+                                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to[k] + col) = get(k);
+                            __syncwarp();
                         }
-                        __syncwarp();
-                        const int col = c + lane % 4 * 8;
+                    } else {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (to[k] >= 0 && col < a.cache.head_dim)
-                                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to[k] + col) = get(k);
-                        __syncwarp();
-                    }
-                } else {
+                        for (int c = 0; c < 64; c += 16) {
 #pragma unroll
-                    for (int c = 0; c < DPAD; c += 16) {
-                        const uint32_t* const o = all + c;
+                            for (int i = 0; i < 4; ++i)
+                                put(i, make_uint4(o[c + i * 4], o[c + i * 4 + 1], o[c + i * 4 + 2], o[c + i * 4 + 3]));
+                            __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) put(i, make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]));
-                        __syncwarp();
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int to = row0 + k * 8 + lane / 4;
-                            if (to < done.rows)
-                                *reinterpret_cast<uint4*>(&block->o[to][c + lane % 4 * 4]) = get(k);
+                            for (int k = 0; k < 4; ++k) {
+                                const int r2 = row0 + k * 8 + lane / 4;
+                                if (r2 < it.rows) *reinterpret_cast<uint4*>(&block->o[r2][c0 + c + lane % 4 * 4]) = get(k);
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
                     }
                 }
                 if (real && !(begins && ends)) {
@@ -811,14 +846,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 }
                 if (sm.odd) {
                     __syncwarp();  // orders the row's stores by other lanes before this one's
-                    if (real && begins && ends) add_odd_values<T, QUANT, T>(a, done, t0, t_end, r, static_cast<T*>(a.out) + mine);
-                    else if (real) add_odd_values<T, QUANT, float>(a, done, t0, t_end, r, block->o[r]);
+                    if (real && begins && ends) add_odd_values<T, QUANT, T>(a, it, t0, t_end, r, static_cast<T*>(a.out) + mine);
+                    else if (real) add_odd_values<T, QUANT, float>(a, it, t0, t_end, r, block->o[r]);
                 }
             }
             tmem_fence_before();
             if (begins && !ends && row == 0 && h == 0)
-                a.joins[blockIdx.x] = make_int4(done.b, done.rt, done.h, owner(share, after + (done.tiles - t_end) - 1));
+                a.joins[blockIdx.x] = make_int4(it.b, it.rt, it.h, owner(share, next_at + (it.tiles - t_end) - 1));
             if (!more) break;
+            it = following;
+            at = next_at;
+            share.t = 0;
         }
         asm volatile("bar.arrive 2, 416;" ::: "memory");
     }
