@@ -26,10 +26,11 @@ struct AttnArgs {
 // the q heads that share it, token by token: row r is token r / group, head
 // r % group of the group. A tile of TILE rows against one kv head is an item;
 // its keys come in tiles of BN. All items' key tiles, in the order (sequence,
-// row tile, kv head, key tile), form one list, and CTA c of N takes the part
-// from c * total / N up to (c + 1) * total / N of it. So every CTA gets the
-// same number of key tiles whatever the sequences' lengths are, and no CTA
-// holds parts of more than one item that it does not own whole at each end.
+// row tile, kv head, key tile), form one list, in which COST places that stand
+// for what an item costs by itself precede its tiles. CTA c of N takes the
+// part from c * total / N up to (c + 1) * total / N of it. So every CTA gets
+// the same work whatever the sequences' lengths are, and a CTA shares at most
+// two items with others, the one at its part's begin and the one at its end.
 struct Item {
     int b, rt, h;           // sequence, row tile, kv head
     int first, n, kv;       // the sequence's first new token, new and cached tokens
@@ -61,10 +62,10 @@ __device__ __forceinline__ int key_tile(const Item& it, int t) {
 template <int TILE>
 __device__ __forceinline__ int row_tiles(const AttnArgs& a, int n) { return (n * a.group + TILE - 1) / TILE; }
 
-// Key tiles of sequence `b` over its row tiles and heads. All lanes of a warp
+// Places of sequence `b` over its row tiles and heads. All lanes of a warp
 // call it, with b = -1 for none: sequences with many row tiles are summed by
 // the whole warp.
-template <int TILE, int BN>
+template <int TILE, int BN, int COST>
 __device__ __forceinline__ int64_t sequence_tiles(const AttnArgs& a, int b) {
     Item it;
     it.n = 0;
@@ -78,7 +79,7 @@ __device__ __forceinline__ int64_t sequence_tiles(const AttnArgs& a, int b) {
     if (nrt <= 4) {
         for (it.rt = 0; it.rt < nrt; ++it.rt) {
             item_geometry<TILE, BN>(a, it);
-            sum += it.tiles;
+            sum += it.tiles + COST;
         }
     }
     const int lane = static_cast<int>(threadIdx.x & 31);
@@ -91,7 +92,7 @@ __device__ __forceinline__ int64_t sequence_tiles(const AttnArgs& a, int b) {
         int64_t s = 0;
         for (o.rt = lane; o.rt < tiles; o.rt += 32) {
             item_geometry<TILE, BN>(a, o);
-            s += o.tiles;
+            s += o.tiles + COST;
         }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
@@ -100,12 +101,27 @@ __device__ __forceinline__ int64_t sequence_tiles(const AttnArgs& a, int b) {
     return sum * a.cache.kv_heads;
 }
 
-// This CTA's part of the list, and the item and key tile where it begins.
+// This CTA's part of the list, and the item that it is at.
+template <int COST>
 struct Share {
     int64_t begin, end, total;
     int ctas;  // CTAs that take part
     Item it;
-    int t;  // key tile within the item
+    int64_t item_at;  // where the item begins in the list
+
+    // The part's tiles of the item: first() .. last() - 1.
+    __device__ __forceinline__ int first() const {
+        const int64_t t = begin - item_at - COST;
+        return t > 0 ? static_cast<int>(t) : 0;
+    }
+    __device__ __forceinline__ int last() const {
+        const int64_t t = end - item_at - COST;
+        return t < it.tiles ? static_cast<int>(t) : it.tiles;
+    }
+    // The last CTA that has a tile of the item.
+    __device__ __forceinline__ int last_cta() const {
+        return static_cast<int>(((item_at + COST + it.tiles) * ctas - 1) / total);
+    }
 };
 
 struct ShareScratch {
@@ -115,16 +131,16 @@ struct ShareScratch {
 };
 
 // All threads of the CTA call it (THREADS a multiple of 32). False when this
-// CTA has nothing to do.
-template <int TILE, int BN, int THREADS>
-__device__ bool find_share(const AttnArgs& a, int per_cta, ShareScratch& sm, Share& out) {
+// CTA has nothing to do. No CTA takes less than `per_cta` places if it can help it.
+template <int TILE, int BN, int COST, int THREADS>
+__device__ bool find_share(const AttnArgs& a, int per_cta, ShareScratch& sm, Share<COST>& out) {
     constexpr int WARPS = THREADS / 32;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
     const int chunks = (a.seqs.batch + THREADS - 1) / THREADS;
     int64_t mine = 0, total = 0;
     for (int i = 0; i < chunks; ++i) {
         const int b = i * THREADS + tid;
-        mine = sequence_tiles<TILE, BN>(a, b < a.seqs.batch ? b : -1);
+        mine = sequence_tiles<TILE, BN, COST>(a, b < a.seqs.batch ? b : -1);
         total += mine;
     }
 #pragma unroll
@@ -144,7 +160,7 @@ __device__ bool find_share(const AttnArgs& a, int per_cta, ShareScratch& sm, Sha
     int64_t before = 0;
     for (int i = 0; i < chunks; ++i) {
         const int b = i * THREADS + tid;
-        if (chunks > 1) mine = sequence_tiles<TILE, BN>(a, b < a.seqs.batch ? b : -1);
+        if (chunks > 1) mine = sequence_tiles<TILE, BN, COST>(a, b < a.seqs.batch ? b : -1);
         int64_t incl = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -174,18 +190,21 @@ __device__ bool find_share(const AttnArgs& a, int per_cta, ShareScratch& sm, Sha
     const int last = row_tiles<TILE>(a, it.n) - 1;
     for (it.rt = 0;; ++it.rt) {
         item_geometry<TILE, BN>(a, it);
-        const int64_t all = static_cast<int64_t>(it.tiles) * a.cache.kv_heads;
+        const int64_t all = static_cast<int64_t>(it.tiles + COST) * a.cache.kv_heads;
         if (at < all || it.rt >= last) break;
         at -= all;
     }
-    it.h = static_cast<int>(at / it.tiles);
-    out.t = static_cast<int>(at - static_cast<int64_t>(it.h) * it.tiles);
-    return true;
+    it.h = static_cast<int>(at / (it.tiles + COST));
+    out.item_at = out.begin - (at - static_cast<int64_t>(it.h) * (it.tiles + COST));
+    return out.last() > out.first();
 }
 
-// The item behind `it` in the list; false behind the last.
-template <int TILE, int BN>
-__device__ __forceinline__ bool next_item(const AttnArgs& a, Item& it) {
+// Moves on to the next item; false when the part has none of its tiles.
+template <int TILE, int BN, int COST>
+__device__ __forceinline__ bool next_item(const AttnArgs& a, Share<COST>& s) {
+    Item& it = s.it;
+    s.item_at += it.tiles + COST;
+    if (s.item_at + COST >= s.end) return false;
     if (++it.h < a.cache.kv_heads) return true;
     it.h = 0;
     if (++it.rt < row_tiles<TILE>(a, it.n)) {
@@ -202,11 +221,6 @@ __device__ __forceinline__ bool next_item(const AttnArgs& a, Item& it) {
         }
     }
     return false;
-}
-
-// The CTA that tile `t` of the list belongs to.
-__device__ __forceinline__ int owner(const Share& s, int64_t t) {
-    return static_cast<int>(((t + 1) * s.ctas - 1) / s.total);
 }
 
 // ---------------------------------------------------------------- partials
@@ -249,14 +263,15 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, const Item& it, int
 }
 
 // Joins the parts of the items that several CTAs took: CTA (c, y) the rows
-// [y * 4 WARPS...) of the item that CTA c of the grid before it began.
-template <typename T, int ROWS, int DPAD>
+// [y * EACH, (y + 1) * EACH) of the item that CTA c of the grid before it began.
+// Bound by the parts' bytes, so a thread asks for its rows of a part at once.
+template <typename T, int ROWS, int DPAD, int EACH>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     pdl_enter();
     const int4 j = a.joins[blockIdx.x];
     if (j.x < 0) return;
     using Block = PartialBlock<ROWS, DPAD>;
-    constexpr int LANES = DPAD / 4, STEP = 128 / LANES;
+    constexpr int LANES = DPAD / 4, STEP = 128 / LANES, TIMES = EACH / STEP;
     Item it;
     it.b = j.x;
     it.rt = j.y;
@@ -264,30 +279,47 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     new_tokens(a.seqs, it.b, it.first, it.n);
     it.row0 = it.rt * ROWS;
     it.rows = min(ROWS, it.n * a.group - it.row0);
-    const int r = static_cast<int>(blockIdx.y) * STEP + static_cast<int>(threadIdx.x) / LANES;
+    const int r0 = static_cast<int>(blockIdx.y) * EACH + static_cast<int>(threadIdx.x) / LANES;
     const int c = static_cast<int>(threadIdx.x) % LANES * 4;
-    if (r >= it.rows) return;
-    const Block* const first = reinterpret_cast<const Block*>(a.partial) + 2 * blockIdx.x + 1;
-    const Block* const others = reinterpret_cast<const Block*>(a.partial) + 2 * (blockIdx.x + 1);
-    const int n = j.w - static_cast<int>(blockIdx.x);  // CTAs behind the first
-    float top = first->m[r];
-    for (int i = 0; i < n; ++i) top = fmaxf(top, others[2 * i].m[r]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float f = ex2(first->m[r] - ref), sum = f * first->l[r];
-    float4 v = *reinterpret_cast<const float4*>(&first->o[r][c]);
-    float4 acc = make_float4(f * v.x, f * v.y, f * v.z, f * v.w);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const Block& b = others[2 * i];
-        f = ex2(b.m[r] - ref);
-        v = *reinterpret_cast<const float4*>(&b.o[r][c]);
-        sum = fmaf(f, b.l[r], sum);
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
+    if (r0 >= it.rows) return;
+    // block 2c + 1 of the first CTA, blocks 2i of those behind it
+    const Block* const own = reinterpret_cast<const Block*>(a.partial) + 2 * blockIdx.x + 1;
+    const int n = j.w - static_cast<int>(blockIdx.x);
+    float top[TIMES], sum[TIMES];
+    float4 acc[TIMES];
+#pragma unroll
+    for (int i = 0; i < TIMES; ++i) {
+        const int r = min(r0 + i * STEP, it.rows - 1);
+        top[i] = own->m[r];
+        sum[i] = own->l[r];
+        acc[i] = *reinterpret_cast<const float4*>(&own->o[r][c]);
     }
-    write_row<T>(a, it, r, c, acc, sum);
+    for (int k = 0; k < n; ++k) {
+        const Block& b = own[2 * k + 1];
+        float m[TIMES], l[TIMES];
+        float4 v[TIMES];
+#pragma unroll
+        for (int i = 0; i < TIMES; ++i) {
+            const int r = min(r0 + i * STEP, it.rows - 1);
+            m[i] = b.m[r];
+            l[i] = b.l[r];
+            v[i] = *reinterpret_cast<const float4*>(&b.o[r][c]);
+        }
+#pragma unroll
+        for (int i = 0; i < TIMES; ++i) {
+            const float mn = fmaxf(top[i], m[i]), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = ex2(top[i] - ref), g = ex2(m[i] - ref);
+            top[i] = mn;
+            sum[i] = fmaf(g, l[i], f * sum[i]);
+            acc[i].x = fmaf(g, v[i].x, f * acc[i].x);
+            acc[i].y = fmaf(g, v[i].y, f * acc[i].y);
+            acc[i].z = fmaf(g, v[i].z, f * acc[i].z);
+            acc[i].w = fmaf(g, v[i].w, f * acc[i].w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TIMES; ++i)
+        if (r0 + i * STEP < it.rows) write_row<T>(a, it, r0 + i * STEP, c, acc[i], sum[i]);
 }
 
 }  // namespace ako_b200

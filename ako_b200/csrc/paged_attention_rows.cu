@@ -14,9 +14,9 @@ int launch(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
     if (rc) return rc;
     rc = launch_ex(attn_rows_kernel<T, QUANT, DPAD, NT>, dim3(p.ctas), dim3(kRowsThreads), Shape::kSmem, 1, st, a, name);
     if (rc) return rc;
-    constexpr int STEP = 128 / (DPAD / 4);
-    return launch_ex(attn_join_kernel<T, Shape::kRows, DPAD>, dim3(p.ctas, (Shape::kRows + STEP - 1) / STEP), dim3(128), 0,
-                     1, st, a, name);
+    constexpr int EACH = 8;  // rows of a CTA that joins
+    return launch_ex(attn_join_kernel<T, Shape::kRows, DPAD, EACH>, dim3(p.ctas, Shape::kRows / EACH), dim3(128), 0, 1, st,
+                     a, name);
 }
 
 template <typename T, bool QUANT, int DPAD, int NT>

@@ -24,6 +24,7 @@ constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kWarpKeys = 16;
 constexpr int kRowsKeys = kRowsWarps * kWarpKeys;  // keys of a tile
+constexpr int kRowsCost = 1;                       // tiles that an item's begin and end take as long as
 
 // 16-byte asynchronous copy; zeros instead when `real` is false.
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool real) {
@@ -155,16 +156,15 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
     const int dim = a.cache.head_dim;
 
     if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    Share share;
-    if (!find_share<ROWS, kRowsKeys, kRowsThreads>(a, 1, scratch, share)) return;
+    Share<kRowsCost> share;
+    if (!find_share<ROWS, kRowsKeys, kRowsCost, kRowsThreads>(a, kRowsCost + 1, scratch, share)) return;
     Item& it = share.it;
 
     uint8_t* const ring = smem + warp * (STAGES * Shape::kStageBytes);
     const uint32_t ring_addr = smem_addr(ring);
 
-    int64_t at = share.begin;
     while (true) {
-        const int t_end = static_cast<int>(min(static_cast<int64_t>(it.tiles), share.t + (share.end - at)));
+        const int t0 = share.first(), t_end = share.last();
 
         // ------------------------------------------------ keys under way
         // Lanes 0-15 look after the 16 keys' rows of K, lanes 16-31 of V.
@@ -207,9 +207,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
             }
             cp_async_commit();
         };
-        look_up(share.t);
+        look_up(t0);
 #pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) issue(share.t + i, i);
+        for (int i = 0; i < STAGES - 1; ++i) issue(t0 + i, i);
 
         // ------------------------------------------------------------ rows
         for (int r = warp; r < ROWS; r += kRowsWarps) {
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
 
         // ------------------------------------------------------------ keys
         int stage = 0;
-        for (int t = share.t; t < t_end; ++t) {
+        for (int t = t0; t < t_end; ++t) {
             const int to = stage == 0 ? STAGES - 1 : stage - 1;
             issue(t + STAGES - 1, to);
             cp_async_wait<STAGES - 1>();
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                 }
             }
         __syncthreads();
-        const bool begins = share.t == 0, ends = t_end == it.tiles;
+        const bool begins = t0 == 0, ends = t_end == it.tiles;
         Block* const block = reinterpret_cast<Block*>(a.partial) + 2 * blockIdx.x + (begins ? 1 : 0);
         constexpr int LANES = DPAD / 4;  // of a row
         for (int r = tid / LANES; r < it.rows; r += kRowsThreads / LANES) {
@@ -548,11 +548,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                 }
             }
         }
-        at += t_end - share.t;
-        if (begins && !ends && tid == 0)
-            a.joins[blockIdx.x] = make_int4(it.b, it.rt, it.h, owner(share, at + (it.tiles - t_end) - 1));
-        if (at >= share.end || !next_item<ROWS, kRowsKeys>(a, it)) return;
-        share.t = 0;
+        if (begins && !ends && tid == 0) a.joins[blockIdx.x] = make_int4(it.b, it.rt, it.h, share.last_cta());
+        if (!next_item<ROWS, kRowsKeys>(a, share)) return;
         __syncthreads();  // before the rings and the rows are filled again
     }
 }

@@ -59,9 +59,9 @@ int launch(const TilesArgs& t, const AttnPlan& p, cudaStream_t st) {
     if (rc) return rc;
     rc = launch_ex(kernel, dim3(p.ctas), dim3(kTilesThreads), Shape::kSmem, 1, st, t, name);
     if (rc) return rc;
-    constexpr int STEP = 128 / (DPAD / 4);
-    return launch_ex(attn_join_kernel<T, kTilesRows, DPAD>, dim3(p.ctas, kTilesRows / STEP), dim3(128), 0, 1, st, t.a,
-                     name);
+    constexpr int EACH = 32;  // rows of a CTA that joins
+    return launch_ex(attn_join_kernel<T, kTilesRows, DPAD, EACH>, dim3(p.ctas, kTilesRows / EACH), dim3(128), 0, 1, st,
+                     t.a, name);
 }
 
 template <typename T>

@@ -41,6 +41,7 @@ namespace ako_b200 {
 constexpr int kTilesThreads = 512;
 constexpr int kTilesRows = 256;
 constexpr int kTilesKeys = 128;
+constexpr int kTilesCost = 4;  // tiles that an item's begin and end take as long as
 constexpr int kEarly = 96;  // keys whose weights are handed on before the tile's others
 // Tiles whose key data are kept: the loading warps find a tile's keys one tile
 // before they bring them, at most STAGES + 2 tiles ahead of the softmax.
@@ -324,8 +325,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     const uint32_t polls = args.wait_polls;
 
     if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    Share share;
-    if (!find_share<kTilesRows, kTilesKeys, kTilesThreads>(a, 1, sm.scratch, share)) return;
+    Share<kTilesCost> share;
+    if (!find_share<kTilesRows, kTilesKeys, kTilesCost, kTilesThreads>(a, kTilesCost + 1, sm.scratch, share)) return;
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&sm.k_full[i], QUANT ? 128 : 64);
@@ -351,14 +352,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     tmem_fence_after();
     const uint32_t tmem = sm.tmem;
     Item& it = share.it;
-    int64_t at = share.begin;
-    auto part_end = [&] { return static_cast<int>(min(static_cast<int64_t>(it.tiles), share.t + (share.end - at))); };
     // moves on to the next item; false when the share is done
-    auto advance = [&](int t_end) {
-        at += t_end - share.t;
-        share.t = 0;
-        return at < share.end && next_item<kTilesRows, kTilesKeys>(a, it);
-    };
+    auto advance = [&] { return next_item<kTilesRows, kTilesKeys>(a, share); };
 
     if (wg == 3) {
         // ---------------------------------------------------------- products
@@ -408,21 +403,21 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             }
         };
         do {
-            const int t_end = part_end();
+            const int t0 = share.first(), t_end = share.last();
             const int halves = it.rows > 128 ? 2 : 1;
-            for (int t = share.t; t < t_end && ok; ++t, ++n) {
-                if (t == share.t) {
+            for (int t = t0; t < t_end && ok; ++t, ++n) {
+                if (t == t0) {
                     await(&sm.q_full[0], nq[0]++);
                     if (halves == 2) await(&sm.q_full[1], nq[1]++);
                 }
                 await(&sm.k_full[n % STAGES], n / STAGES);
                 const bool whole = whole_tile(a, it, key_tile(it, t) * kTilesKeys);
-                order_copies(whole && t > share.t);  // q is copied too
+                order_copies(whole && t > t0);  // q is copied too
                 const uint64_t k = k_desc + (n % STAGES) * Shape::kOperand / 16;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (h >= halves || !ok) break;
-                    if (t > share.t) weigh(h, n - 1, t - 1 > share.t);
+                    if (t > t0) weigh(h, n - 1, t - 1 > t0);
                     if (!ok) break;
                     if (elect_one()) {
                         const uint64_t q = q_desc + h * Shape::kOperand / 16;
@@ -436,7 +431,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                     ++ns[h];
                 }
                 if (elect_one()) {
-                    if (t > share.t) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
+                    if (t > t0) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
                     mma_commit(&sm.k_empty[n % STAGES]);
                 }
                 before = whole;
@@ -444,11 +439,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (h >= halves || !ok) break;
-                weigh(h, n - 1, t_end - 1 > share.t);
+                weigh(h, n - 1, t_end - 1 > t0);
                 if (elect_one()) mma_commit(&sm.o_full[h]);
             }
             if (elect_one()) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
-            if (!advance(t_end)) break;
+            if (!advance()) break;
         } while (ok);
         // nothing of this CTA's is under way when it gives its tensor memory back
         if (elect_one()) mma_commit(&sm.drained);
@@ -472,14 +467,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         };
         // The table entries of a tile's keys are asked for ahead of the tile (by two tiles in an
         // e4m3 cache, whose scales are asked for by one), so that it does not wait for them.
-        int t_end = part_end();
-        int t = share.t;
+        int t = share.first(), t_end = share.last();
         // moves on to the next tile; false behind the last
         auto step = [&] {
             if (++t < t_end) return true;
-            if (!advance(t_end)) return false;
-            t = 0;
-            t_end = part_end();
+            if (!advance()) return false;
+            t = share.first();
+            t_end = share.last();
             return true;
         };
         auto key0 = [&] { return key_tile(it, t) * kTilesKeys; };
@@ -644,11 +638,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
         };
         bool loaded = false;
         while (true) {
-            const int t0 = share.t, t_end = part_end();
+            const int t0 = share.first(), t_end = share.last();
             if (it.rows <= h * 128) {  // the other half's rows are all there are
                 n += t_end - t0;
                 loaded = false;
-                if (!advance(t_end)) break;
+                if (!advance()) break;
                 continue;
             }
             if (!loaded) load_q(it);
@@ -658,16 +652,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             const float my_factor = factor;
             // The next item and its rows of q, which take the place of this one's once the last scores
             // are there.
-            Item following;
+            Share<kTilesCost> following = share;
             bool more = false;
-            int64_t next_at = at;
             loaded = false;
             auto prepare_next = [&] {
-                next_at = at + (t_end - t0);
-                following = it;
-                more = next_at < share.end && next_item<kTilesRows, kTilesKeys>(a, following);
-                if (more && following.rows > h * 128) {
-                    load_q(following);
+                more = next_item<kTilesRows, kTilesKeys>(a, following);
+                if (more && following.it.rows > h * 128) {
+                    load_q(following.it);
                     loaded = true;
                 }
             };
@@ -773,10 +764,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 mbar_arrive(&sm.p_full[h][1]);
             }
             if (!ok) {
+                following = share;
+                more = next_item<kTilesRows, kTilesKeys>(a, following);
                 loaded = false;
-                next_at = at + (t_end - t0);
-                following = it;
-                more = next_at < share.end && next_item<kTilesRows, kTilesKeys>(a, following);
             }
             ok = ok && tile_wait(sm, &sm.o_full[h], no++ & 1, polls);
             ok = __all_sync(0xffffffffu, ok);
@@ -852,11 +842,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             }
             tmem_fence_before();
             if (begins && !ends && row == 0 && h == 0)
-                a.joins[blockIdx.x] = make_int4(it.b, it.rt, it.h, owner(share, next_at + (it.tiles - t_end) - 1));
+                a.joins[blockIdx.x] = make_int4(it.b, it.rt, it.h, share.last_cta());
             if (!more) break;
-            it = following;
-            at = next_at;
-            share.t = 0;
+            share = following;
         }
         asm volatile("bar.arrive 2, 416;" ::: "memory");
     }
