@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             uint64_t* const empty = values ? sm.v_empty : sm.k_empty;
             Place p0 = load.look_up(it, key0()), p1 = load.look_up(it, key0(), 32);
             bool more = true;
-            for (uint32_t n = 0; more; ++n) {
+            uint32_t n = 0;
+            for (; more; ++n) {
                 const int st = n % STAGES;
                 const Place now0 = p0, now1 = p1;
                 more = step();
@@ -526,6 +527,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                     fence_proxy_async_smem();
                     mbar_arrive(&full[st]);
                 }
+            }
+            if (!ok) {  // copies by tensor map that no one waits for any more land before the CTA ends
+                const volatile int never = 0;
+                for (uint32_t u = n > STAGES ? n - STAGES : 0; u < n; ++u)
+                    wait_bounded(&full[u % STAGES], (u / STAGES) & 1, kDrainPolls, &never);
             }
         } else {
             typename Loader::Place place = load.look_up(it, key0());

@@ -18,7 +18,11 @@ norm/residual order as the reference; the layout is chosen for B200:
 * grouped-query attention goes through SDPA with ``enable_gqa`` instead of
   materializing repeated heads (``ako/models/decoder.py:180-182``).
 
-GEMMs and attention are torch's (cuBLAS / SDPA), as config 5 specifies.
+GEMMs and attention are torch's (cuBLAS / SDPA), as config 5 specifies. With a
+:class:`PagedKVCache` (``Decoder.new_paged_cache``) attention runs on this
+package's kernels instead: keys and values live in pages, as they are or in
+e4m3, chunks of tokens may follow a filled cache, and a sliding window with
+first tokens that stay visible is possible.
 ``backend="torch"`` runs the same stack with the unfused reference math for
 RMSNorm, RoPE and SwiGLU (AKO's own ``ako.ops.*_ref``), for comparison.
 """
@@ -33,6 +37,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from ako_b200 import _native, kernels
+from ako_b200.paged import (PagedBatch, PagedKV, kv_cache_write_cuda_sm100,
+                            paged_attention_cuda_sm100)
 from ako_b200.reference import ops as reference_ops
 
 Backend = Literal["b200", "torch"]
@@ -87,6 +93,41 @@ class KVCache:
         return self.k[layer][:, :, :end], self.v[layer][:, :, :end]
 
 
+class PagedKVCache:
+    """Per-layer paged keys and values (:class:`ako_b200.PagedKV`) of a batch of sequences that grow together.
+
+    One page table serves all layers; each sequence owns ``ceil(max_len /
+    page_size)`` pages. ``kv_dtype`` is the element type of the cache: ``dtype``
+    (float16 or bfloat16) or ``torch.float8_e4m3fn``. ``window`` and ``sinks``
+    are those of :func:`ako_b200.paged_attention_cuda_sm100`.
+    """
+
+    def __init__(self, config: ModelConfig, batch: int, max_len: int, *, device, dtype, page_size: int = 64,
+                 kv_dtype: torch.dtype | None = None, window: int = 0, sinks: int = 0) -> None:
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"PagedKVCache: attention over pages supports float16/bfloat16 models, got {dtype}")
+        pages = -(-max_len // page_size)
+        self.layers = [PagedKV.empty(batch * pages, config.n_kv_heads, page_size, config.head_dim,
+                                     dtype=kv_dtype or dtype, device=device) for _ in range(config.n_layers)]
+        self.kv_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.batch = PagedBatch(torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages),
+                                self.kv_lens)
+        self.window, self.sinks = window, sinks
+        self.length = 0
+        self.max_len = max_len
+
+    def extend(self, n: int) -> None:
+        """Make room for ``n`` more positions of every sequence (the step's new tokens)."""
+        if self.length + n > self.max_len:
+            raise ValueError(f"KV cache holds {self.max_len} positions, asked for {self.length + n}")
+        self.kv_lens.fill_(self.length + n)
+
+    def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Store the new tokens' rotated keys and values, then attend: ``(batch, n, heads, head_dim)`` tensors."""
+        kv_cache_write_cuda_sm100(k, v, self.layers[layer], self.batch)
+        return paged_attention_cuda_sm100(q, self.layers[layer], self.batch, window=self.window, sinks=self.sinks)
+
+
 class DecoderLayer(nn.Module):
     def __init__(self, cfg: ModelConfig, backend: Backend) -> None:
         super().__init__()
@@ -135,7 +176,7 @@ class DecoderLayer(nn.Module):
         return reference_ops().swiglu_ref(gate, up)
 
     # --------------------------------------------------------------- block
-    def forward(self, x, residual, cos, sin, cache: KVCache | None, layer: int):
+    def forward(self, x, residual, cos, sin, cache: KVCache | PagedKVCache | None, layer: int):
         cfg = self.cfg
         b, s, _ = x.shape
         h, residual = self._norm(x, residual, self.input_norm_weight)
@@ -143,6 +184,9 @@ class DecoderLayer(nn.Module):
         q = qkv[..., : self.q_dim].view(b, s, cfg.n_heads, cfg.head_dim)
         k = qkv[..., self.q_dim : self.q_dim + self.kv_dim].view(b, s, cfg.n_kv_heads, cfg.head_dim)
         v = qkv[..., self.q_dim + self.kv_dim :].view(b, s, cfg.n_kv_heads, cfg.head_dim)
+        if isinstance(cache, PagedKVCache):
+            q, k = self._rope(q, k, cos, sin, None)
+            return self._finish(cache.attend(layer, q, k, v).reshape(b, s, self.q_dim), residual)
         start = cache.length if cache is not None else 0
         if s > 1 and start > 0:
             raise NotImplementedError("chunked prefill onto a non-empty cache is not supported")
@@ -158,20 +202,22 @@ class DecoderLayer(nn.Module):
         attn = F.scaled_dot_product_attention(
             q.transpose(1, 2), keys, values, is_causal=s > 1 and start == 0, enable_gqa=True
         )
-        out = self.o_proj(attn.transpose(1, 2).reshape(b, s, self.q_dim))
+        return self._finish(attn.transpose(1, 2).reshape(b, s, self.q_dim), residual)
+
+    def _finish(self, attn, residual):
+        out = self.o_proj(attn)
         h, residual = self._norm(out, residual, self.post_attention_norm_weight)
         return self.down_proj(self._swiglu(self.gate_up_proj(h))), residual
 
-
-    def forward_static(self, x, residual, cos, sin, cache: "KVCache", layer: int, pos: torch.Tensor,
-                       mask: torch.Tensor):
+    def forward_static(self, x, residual, cos, sin, cache: "KVCache | PagedKVCache", layer: int, pos: torch.Tensor,
+                       mask: torch.Tensor | None):
         """One decode step with shapes fixed for CUDA-graph capture.
 
         ``pos`` is a one-element device tensor holding the write position; the
         new key and value go into the cache with ``index_copy_`` at ``pos`` and
         attention runs over the whole preallocated cache under ``mask``
         (``(1, 1, 1, max_len)``, true up to ``pos``), so nothing depends on
-        host-side lengths.
+        host-side lengths. A paged cache has its own lengths on the device.
         """
         cfg = self.cfg
         b = x.shape[0]
@@ -181,13 +227,13 @@ class DecoderLayer(nn.Module):
         k = qkv[..., self.q_dim : self.q_dim + self.kv_dim].view(b, 1, cfg.n_kv_heads, cfg.head_dim)
         v = qkv[..., self.q_dim + self.kv_dim :].view(b, 1, cfg.n_kv_heads, cfg.head_dim)
         q, k = self._rope(q, k, cos, sin, None)
+        if isinstance(cache, PagedKVCache):
+            return self._finish(cache.attend(layer, q, k, v).reshape(b, 1, self.q_dim), residual)
         cache.k[layer].index_copy_(2, pos, k.transpose(1, 2))
         cache.v[layer].index_copy_(2, pos, v.transpose(1, 2))
         attn = F.scaled_dot_product_attention(q.transpose(1, 2), cache.k[layer], cache.v[layer], attn_mask=mask,
                                               enable_gqa=True)
-        out = self.o_proj(attn.transpose(1, 2).reshape(b, 1, self.q_dim))
-        h, residual = self._norm(out, residual, self.post_attention_norm_weight)
-        return self.down_proj(self._swiglu(self.gate_up_proj(h))), residual
+        return self._finish(attn.transpose(1, 2).reshape(b, 1, self.q_dim), residual)
 
 
 class Decoder(nn.Module):
@@ -214,12 +260,23 @@ class Decoder(nn.Module):
         p = self.embed.weight
         return KVCache(self.cfg, batch, max_len or self.cfg.max_seq_len, device=p.device, dtype=p.dtype)
 
-    def hidden(self, ids: torch.Tensor, cache: KVCache | None = None) -> torch.Tensor:
+    def new_paged_cache(self, batch: int, max_len: int | None = None, **kwargs) -> PagedKVCache:
+        """A :class:`PagedKVCache`; ``kwargs``: its ``page_size``, ``kv_dtype``, ``window`` and ``sinks``."""
+        if self.backend != "b200":
+            raise ValueError("a paged cache needs backend='b200'")
+        p = self.embed.weight
+        return PagedKVCache(self.cfg, batch, max_len or self.cfg.max_seq_len, device=p.device, dtype=p.dtype, **kwargs)
+
+    def hidden(self, ids: torch.Tensor, cache: KVCache | PagedKVCache | None = None) -> torch.Tensor:
         """Final-normed hidden states ``(batch, seq, hidden)`` of token ids ``(batch, seq)``."""
         s = ids.shape[1]
         start = cache.length if cache is not None else 0
         cos, sin = self.rope_tables(ids.device)
         cos, sin = cos[start:start + s], sin[start:start + s]
+        if isinstance(cache, PagedKVCache):
+            if self.backend != "b200":
+                raise ValueError("a paged cache needs backend='b200'")
+            cache.extend(s)
         x = self.embed(ids)
         residual = None
         for i, layer in enumerate(self.layers):
@@ -232,7 +289,7 @@ class Decoder(nn.Module):
             out, _ = reference_ops().rmsnorm_residual_ref(x, residual, self.final_norm_weight, self.cfg.eps)
         return out
 
-    def forward(self, ids: torch.Tensor, cache: KVCache | None = None) -> torch.Tensor:
+    def forward(self, ids: torch.Tensor, cache: KVCache | PagedKVCache | None = None) -> torch.Tensor:
         """Logits of the last position of each sequence, ``(batch, vocab)``."""
         return self.lm_head(self.hidden(ids, cache)[:, -1])
 
@@ -244,11 +301,13 @@ class GraphDecoder:
     replay: one launch instead of ~55, so the step runs at device speed rather
     than at the speed of Python issuing kernels. The position lives on the
     device and advances inside the graph; attention covers the preallocated
-    cache under a position mask, so the graph is valid for every step. Tokens
-    are written to ``tokens[:, step]`` on the device.
+    cache under a position mask, or a paged cache up to the device's lengths, so
+    the graph is valid for every step. Tokens are written to ``tokens[:, step]``
+    on the device.
     """
 
-    def __init__(self, model: "Decoder", cache: KVCache, first_token: torch.Tensor, steps: int) -> None:
+    def __init__(self, model: "Decoder", cache: KVCache | PagedKVCache, first_token: torch.Tensor,
+                 steps: int) -> None:
         self.model = model
         self.cache = cache
         dev = first_token.device
@@ -266,7 +325,11 @@ class GraphDecoder:
         cos_full, sin_full = m.rope_tables(self.tok.device)
         cos = cos_full.index_select(0, self.pos)
         sin = sin_full.index_select(0, self.pos)
-        mask = (self.arange <= self.pos).view(1, 1, 1, -1)
+        mask = None
+        if isinstance(self.cache, PagedKVCache):
+            self.cache.kv_lens.copy_((self.pos + 1).expand(self.cache.kv_lens.shape))
+        else:
+            mask = (self.arange <= self.pos).view(1, 1, 1, -1)
         x = m.embed(self.tok)
         residual = None
         for i, layer in enumerate(m.layers):

@@ -427,3 +427,28 @@ def test_on_a_device_that_is_not_current(cuda_device) -> None:
 
 def test_half_steps() -> None:
     assert all(HALF_STEP[t] == torch.finfo(t).eps / 2 for t in HALF_STEP)
+
+
+def test_expired_wait_is_reported_and_never_silent(cuda_device) -> None:
+    """Attention on the tensor cores with a wait limit of 0 polls (measurement build): every wait gives up at once, the
+    rows become NaN, the expiry is recorded, and calls are refused until it is taken."""
+    from ako_b200 import _native
+
+    with _native.measurement() as lib:
+        try:
+            p = Problem(BF16, False, 8, 2, 128, 16, [(70, 300), (90, 90), (1, 40)], True, 30, cuda_device)
+            assert lib.ako_b200_measure_set_wait_polls(0) == 1 << 24
+            out = _run(p)
+            lib.ako_b200_measure_set_wait_polls(1 << 24)
+            torch.cuda.synchronize()
+            assert bool(out.isnan().all())
+            with pytest.raises(RuntimeError, match="bounded wait"):
+                _run(p)
+            with pytest.raises(RuntimeError, match="bounded wait"):
+                kv_cache_read_cuda_sm100(p.kv(), p.batch(), 0, 8)
+            assert _native.take_device_status() == 1
+            assert _native.take_device_status() == 0
+            check_attention(p, _run(p))
+        finally:
+            lib.ako_b200_measure_set_wait_polls(1 << 24)
+    assert _native.take_device_status() == 0
