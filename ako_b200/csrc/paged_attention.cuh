@@ -235,6 +235,11 @@ struct PartialBlock {
     float o[ROWS][DPAD];
 };
 
+// How far (as a power of two) a row's weights may exceed 1 before what they
+// are relative to is moved: 16-bit weights keep their precision, and sums are
+// rescaled rarely.
+constexpr float kGrowth = 8.0f;
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
         // ------------------------------------------------ keys under way
         // Lanes 0-15 look after the 16 keys' rows of K, lanes 16-31 of V.
         const PagedTensor& mine = lane < 16 ? a.cache.k : a.cache.v;
+        const bool one_page = a.cache.page_size % kWarpKeys == 0;
         int next_page = -1, next_slot = 0;
         auto look_up = [&](int t) {
             const int key = key_tile(it, t) * kRowsKeys + warp * kWarpKeys + (lane & 15);
@@ -180,19 +181,43 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
             if (t < t_end) {
                 const int page = next_page, slot = next_slot;
                 look_up(t + 1);
-                const int64_t off = page >= 0 ? mine.offset(page, it.h, slot) : -1;
                 const uint32_t to = ring_addr + stage * Shape::kStageBytes;
+                const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+                constexpr int BYTES = QUANT ? 1 : 2, TAKEN = 32 / CHUNKS;  // rows that the warp takes at once
+                if (one_page && there == 0xffffu) {
+                    // 16 rows of one page, a slot apart: no lane needs another's place.
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const uint8_t* base = static_cast<const uint8_t*>(kv == 0 ? a.cache.k.p : a.cache.v.p);
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const PagedTensor& t = kv == 0 ? a.cache.k : a.cache.v;
+                        const int c = lane % CHUNKS, row = lane / CHUNKS;
+                        const int first = slot - (lane & 15);  // the first key's slot
+                        const uint8_t* from = static_cast<const uint8_t*>(t.p) +
+                                              (t.offset(page, it.h, first + row) * BYTES + c * 16);
+                        const int64_t step = t.slot * (TAKEN * BYTES);
+                        const bool real = c * 16 < dim * BYTES;
 #pragma unroll
-                    for (int i = 0; i < kWarpKeys * CHUNKS / 32; ++i) {
-                        const int row = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
-                        const int64_t o = __shfl_sync(0xffffffffu, off, kv * 16 + row);
-                        const bool real = o >= 0 && c * 16 < dim * (QUANT ? 1 : 2);
-                        const int sc = kv == 0 ? swizzled<QUANT, DPAD, true>(row, c) : swizzled<QUANT, DPAD, false>(row, c);
-                        cp_async16_or_zero(to + (kv * kWarpKeys + row) * ROWB + sc * 16,
-                                           real ? base + o * (QUANT ? 1 : 2) + c * 16 : base, real);
+                        for (int i = 0; i < kWarpKeys / TAKEN; ++i) {
+                            const int r = row + i * TAKEN;
+                            const int sc = kv == 0 ? swizzled<QUANT, DPAD, true>(r, c) : swizzled<QUANT, DPAD, false>(r, c);
+                            cp_async16_or_zero(to + (kv * kWarpKeys + r) * ROWB + sc * 16, real ? from : t.p, real);
+                            from += step;
+                        }
+                    }
+                } else {
+                    const int64_t off = page >= 0 ? mine.offset(page, it.h, slot) : -1;
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const uint8_t* base = static_cast<const uint8_t*>(kv == 0 ? a.cache.k.p : a.cache.v.p);
+#pragma unroll
+                        for (int i = 0; i < kWarpKeys / TAKEN; ++i) {
+                            const int row = i * TAKEN + lane / CHUNKS, c = lane % CHUNKS;
+                            const int64_t o = __shfl_sync(0xffffffffu, off, kv * 16 + row);
+                            const bool real = o >= 0 && c * 16 < dim * BYTES;
+                            const int sc =
+                                kv == 0 ? swizzled<QUANT, DPAD, true>(row, c) : swizzled<QUANT, DPAD, false>(row, c);
+                            cp_async16_or_zero(to + (kv * kWarpKeys + row) * ROWB + sc * 16,
+                                               real ? base + o * BYTES + c * 16 : base, real);
+                        }
                     }
                 }
                 if constexpr (QUANT) {
@@ -201,9 +226,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                     cp_async4_or_zero(to + 2 * kWarpKeys * ROWB + lane * 4,
                                       page >= 0 ? p + st.offset(page, it.h, slot) : p, page >= 0);
                 }
-                const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
                 if (lane == 0)
-                    *reinterpret_cast<volatile uint32_t*>(ring + (stage + 1) * Shape::kStageBytes - 16) = there & 0xffffu;
+                    *reinterpret_cast<volatile uint32_t*>(ring + (stage + 1) * Shape::kStageBytes - 16) = there;
             }
             cp_async_commit();
         };
@@ -271,14 +295,17 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) q_fragment(ks, nt, qf[ks][nt][0], qf[ks][nt][1]);
         }
-        float m[NT][2], l[NT][2], factor[NT][2];
+        // m: what weights are relative to; limit: scores above it move m (m plus a factor of 2^8,
+        // which the 16-bit types have room for)
+        float m[NT][2], limit[NT][2], l[NT][2], factor[NT][2];
         int pos[NT][2];
         float o[KS][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                m[nt][e] = -INFINITY;
+                m[nt][e] = 0.0f;
+                limit[nt][e] = -INFINITY;
                 l[nt][e] = 0.0f;
                 factor[nt][e] = QUANT ? row_factor[nt * 8 + t4 * 2 + e] : 1.0f;
                 pos[nt][e] = row_pos[nt * 8 + t4 * 2 + e];
@@ -383,33 +410,41 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                     }
             }
             bool grew = false;
-            float alpha[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) grew |= x[nt][e] > limit[nt][e & 1];
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(x[nt][e], x[nt][e + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        if (top > limit[nt][e]) {
+                            // nothing has been summed yet where there was no limit
+                            const float alpha = limit[nt][e] == -INFINITY ? 0.0f : ex2(m[nt][e] - top);
+                            m[nt][e] = top;
+                            limit[nt][e] = top + kGrowth;
+                            l[nt][e] *= alpha;
+#pragma unroll
+                            for (int mt = 0; mt < KS; ++mt) {
+                                o[mt][nt][e] *= alpha;
+                                o[mt][nt][e + 2] *= alpha;
+                            }
+                        }
+                    }
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(x[nt][e], x[nt][e + 2]);
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float mn = fmaxf(m[nt][e], top);
-                    const float ref = mn == -INFINITY ? 0.0f : mn;
-                    alpha[nt][e] = ex2(m[nt][e] - ref);
-                    grew |= mn != m[nt][e];
-                    m[nt][e] = mn;
-                    x[nt][e] = ex2(x[nt][e] - ref);
-                    x[nt][e + 2] = ex2(x[nt][e + 2] - ref);
-                    l[nt][e] = fmaf(l[nt][e], alpha[nt][e],
-                                    QUANT ? fmaf(x[nt][e], unscale[0], x[nt][e + 2] * unscale[1]) : x[nt][e] + x[nt][e + 2]);
+                    x[nt][e] = ex2(x[nt][e] - m[nt][e]);
+                    x[nt][e + 2] = ex2(x[nt][e + 2] - m[nt][e]);
+                    l[nt][e] += QUANT ? fmaf(x[nt][e], unscale[0], x[nt][e + 2] * unscale[1]) : x[nt][e] + x[nt][e + 2];
                 }
-            if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-                for (int mt = 0; mt < KS; ++mt)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[mt][nt][e] *= alpha[nt][e & 1];
-            }
             // The weights go to the 16-bit operand type, as the values are; the sum above took them in fp32.
             uint32_t pf[NT][2];
 #pragma unroll
@@ -507,7 +542,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                 s += __shfl_xor_sync(0xffffffffu, s, 16);
                 const int r = nt * 8 + t4 * 2 + e;
                 if (g == 0) {
-                    join_m[warp * ROWS + r] = m[nt][e];
+                    join_m[warp * ROWS + r] = limit[nt][e] == -INFINITY ? -INFINITY : m[nt][e];
                     join_l[warp * ROWS + r] = s;
                 }
                 float* const to = join_o + (warp * ROWS + r) * Shape::kJoinStride;

@@ -51,7 +51,6 @@ constexpr uint32_t kDrainPolls = 1u << 24;
 // Registers per thread of the softmax, loading and issuing warps. The block is
 // launched with 128 a thread, and 2 * 184 + 96 + 48 = 4 * 128.
 constexpr int kSoftmaxRegs = 184, kLoadRegs = 96, kIssueRegs = 48;
-constexpr float kGrowth = 8.0f;  // log2 of the factor by which a maximum may lag
 
 struct TilesArgs {
     // The cache's keys and values as (page, head, slot, column) in boxes of `box` slots and 64
