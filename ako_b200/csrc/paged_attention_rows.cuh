@@ -24,7 +24,7 @@ constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kWarpKeys = 16;
 constexpr int kRowsKeys = kRowsWarps * kWarpKeys;  // keys of a tile
-constexpr int kRowsCost = 1;                       // tiles that an item's begin and end take as long as
+constexpr int kRowsCost = 2;                       // tiles that an item's begin and end take as long as
 
 // 16-byte asynchronous copy; zeros instead when `real` is false.
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool real) {
@@ -65,13 +65,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same_v<T, __half>) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     } else {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
@@ -113,9 +113,11 @@ struct RowsShape {
     static constexpr int kRowBytes = DPAD * (QUANT ? 1 : 2);
     static constexpr int kChunks = kRowBytes / 16;
     static constexpr int kStageBytes = 2 * kWarpKeys * kRowBytes + (QUANT ? 2 * kWarpKeys * 4 : 0) + 16;
-    // Bytes under way per SM are what the rate follows from: 2 CTAs of four
-    // 24 KB rings (16-bit, head 128).
-    static constexpr int kStages = QUANT ? 4 : 3;
+    // Warps on an SM count for more than stages: a warp's 16 keys are a chain of reads, products and
+    // exponentials. Head 128: with 16 bits two CTAs of 3 stages 51 us a batch of 32 contexts of 2048
+    // tokens, three of 2 stages 54, one of 4 stages 64; in e4m3 four CTAs of 3 stages 172 us where
+    // three of 4 take 179, two of 6 216.
+    static constexpr int kStages = 3;
     static constexpr int kRing = kRowsWarps * kStages * kStageBytes;
     static constexpr int kJoinStride = DPAD + 4;  // floats; keeps the four column groups on different banks
     static constexpr int kJoin = kRowsWarps * kRows * (kJoinStride + 2) * 4;
@@ -328,20 +330,25 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
             const uint32_t there = *reinterpret_cast<const volatile uint32_t*>(st + Shape::kStageBytes - 16);
             const int key0 = key_tile(it, t) * kRowsKeys + warp * kWarpKeys;
 
-            float x[NT][4];
+            // A product waits for the one before it on the same sum, and a warp has little else to do
+            // meanwhile: few rows take their scores as two sums, and fragments are read ahead.
+            constexpr int SUMS = NT == 1 ? 2 : 1;
+            float xs[SUMS][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int c = 0; c < SUMS; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[nt][e] = 0.0f;
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) xs[c][nt][e] = 0.0f;
             auto scores = [&](int ks, const uint32_t(&kf)[4]) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     if constexpr (HOLD) {
-                        mma16816<M>(x[nt], kf, qf[ks][nt][0], qf[ks][nt][1]);
+                        mma16816<M>(xs[ks % SUMS][nt], kf, qf[ks][nt][0], qf[ks][nt][1]);
                     } else {
                         uint32_t b0, b1;
                         q_fragment(ks, nt, b0, b1);
-                        mma16816<M>(x[nt], kf, b0, b1);
+                        mma16816<M>(xs[0][nt], kf, b0, b1);
                     }
                 }
             };
@@ -361,14 +368,41 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                     }
                 }
             } else {
+                constexpr int AHEAD = NT <= 2 ? KS : 2;
+                const int row = lane & 15;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    uint32_t kf[4];
-                    const int row = lane & 15;
-                    ldmatrix4(kf, k_addr + row * ROWB + swizzled<QUANT, DPAD, true>(row, 2 * ks + (lane >> 4)) * 16);
-                    scores(ks, kf);
+                for (int k0 = 0; k0 < KS; k0 += AHEAD) {
+                    uint32_t kf[AHEAD][4];
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i)
+                        ldmatrix4(kf[i],
+                                  k_addr + row * ROWB + swizzled<QUANT, DPAD, true>(row, 2 * (k0 + i) + (lane >> 4)) * 16);
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i) scores(k0 + i, kf[i]);
                 }
             }
+            float x[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[nt][e] = SUMS == 2 ? xs[0][nt][e] + xs[SUMS - 1][nt][e] : xs[0][nt][e];
+            // The values of few rows are asked for before the softmax.
+            constexpr int MATRICES = QUANT ? KS / 2 : KS;  // of 16 keys and 16 or 32 columns
+            constexpr int VAHEAD = NT == 1 ? MATRICES : 2;
+            uint32_t vr[VAHEAD][4];
+            auto read_values = [&](int first) {
+#pragma unroll
+                for (int i = 0; i < VAHEAD; ++i) {
+                    if constexpr (QUANT) {
+                        const int r = (lane & 7) + 8 * ((lane >> 3) & 1), c = 2 * (first + i) + (lane >> 4);
+                        ldmatrix4_trans(vr[i], v_addr + r * ROWB + swizzled<QUANT, DPAD, false>(r, c) * 16);
+                    } else {
+                        const int r = (lane & 7) + 8 * (lane >> 4), c = 2 * (first + i) + ((lane >> 3) & 1);
+                        ldmatrix4_trans(vr[i], v_addr + r * ROWB + swizzled<QUANT, DPAD, false>(r, c) * 16);
+                    }
+                }
+            };
+            if constexpr (NT == 1) read_values(0);
 
             // Scores in units of log2(e). A quantised value's scale joins its key's
             // score as a logarithm, so that the weights of the second product,
@@ -493,34 +527,28 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma16816<M>(o[mt][nt], vf, pf[nt][0], pf[nt][1]);
             };
-            if constexpr (QUANT) {
-                // A 16-bit element of V is the pair (2u, 2u + 1) of a tile's 16 head columns:
-                // its transposed matrices give rows 2u and 2u + 1, which are taken as rows
-                // u and u + 8 of the operand.
 #pragma unroll
-                for (int mt = 0; mt < KS; mt += 2) {
-                    uint32_t r[4];
-                    const int row = (lane & 7) + 8 * ((lane >> 3) & 1);
-                    ldmatrix4_trans(r, v_addr + row * ROWB + swizzled<QUANT, DPAD, false>(row, mt + (lane >> 4)) * 16);
+            for (int first = 0; first < MATRICES; first += VAHEAD) {
+                if constexpr (NT != 1) read_values(first);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint32_t vf[4];
+                for (int i = 0; i < VAHEAD; ++i) {
+                    if constexpr (QUANT) {
+                        // A 16-bit element of V is the pair (2u, 2u + 1) of a tile's 16 head columns:
+                        // its transposed matrices give rows 2u and 2u + 1, which are taken as rows
+                        // u and u + 8 of the operand.
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            vf[2 * j] = e4m3x2_to_half2(__byte_perm(r[2 * i + j], 0, 0x4420));
-                            vf[2 * j + 1] = e4m3x2_to_half2(__byte_perm(r[2 * i + j], 0, 0x4431));
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t vf[4];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                vf[2 * e] = e4m3x2_to_half2(__byte_perm(vr[i][2 * k + e], 0, 0x4420));
+                                vf[2 * e + 1] = e4m3x2_to_half2(__byte_perm(vr[i][2 * k + e], 0, 0x4431));
+                            }
+                            values(2 * (first + i) + k, vf);
                         }
-                        values(mt + i, vf);
+                    } else {
+                        values(first + i, vr[i]);
                     }
-                }
-            } else {
-#pragma unroll
-                for (int mt = 0; mt < KS; ++mt) {
-                    uint32_t vf[4];
-                    const int row = (lane & 7) + 8 * (lane >> 4);
-                    ldmatrix4_trans(vf, v_addr + row * ROWB +
-                                            swizzled<QUANT, DPAD, false>(row, 2 * mt + ((lane >> 3) & 1)) * 16);
-                    values(mt, vf);
                 }
             }
             stage = stage == STAGES - 1 ? 0 : stage + 1;
