@@ -16,9 +16,23 @@ namespace {
 
 bool multiple16(int64_t stride, int64_t extent, int es) { return extent <= 1 || ((stride * es) & 15) == 0; }
 
-bool tensor16(const PagedTensor& t, const ako_b200_paged_kv& c, int es) {
-    return aligned16(t.p) && multiple16(t.page, c.num_pages, es) && multiple16(t.head, c.kv_heads, es) &&
-           multiple16(t.slot, c.page_size, es);
+// A tensor's view, strides in units of `unit` bytes (those of axes of one
+// element play no part); false if a stride does not fit.
+bool make_tensor(void* p, const int64_t (&strides)[3], const ako_b200_paged_kv& c, int es, int unit, PagedTensor& out) {
+    const int64_t extents[3] = {c.num_pages, c.kv_heads, c.page_size};
+    uint32_t units[3];
+    for (int i = 0; i < 3; ++i) {
+        if (extents[i] <= 1) {
+            units[i] = 0;
+            continue;
+        }
+        if (strides[i] < 0 || strides[i] > INT64_MAX / 16 || strides[i] * es % unit != 0 ||
+            strides[i] * es / unit > UINT32_MAX)
+            return false;
+        units[i] = static_cast<uint32_t>(strides[i] * es / unit);
+    }
+    out = PagedTensor{p, units[0], units[1], units[2]};
+    return true;
 }
 
 }  // namespace
@@ -47,14 +61,16 @@ int make_cache(const char* op, const ako_b200_paged_kv* c, int dtype, PagedCache
         return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k or v of the cache is a null pointer", op);
     if (e4m3 && (c->k_scale == nullptr || c->v_scale == nullptr))
         return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: an e4m3 cache needs k_scale and v_scale", op);
-    out.k = PagedTensor{c->k, c->k_stride_page, c->k_stride_head, c->k_stride_slot};
-    out.v = PagedTensor{c->v, c->v_stride_page, c->v_stride_head, c->v_stride_slot};
-    out.ks = PagedTensor{c->k_scale, c->ks_stride_page, c->ks_stride_head, c->ks_stride_slot};
-    out.vs = PagedTensor{c->v_scale, c->vs_stride_page, c->vs_stride_head, c->vs_stride_slot};
-    if (!e4m3) out.ks.p = out.vs.p = nullptr;
-    if (!tensor16(out.k, *c, cache_es) || !tensor16(out.v, *c, cache_es))
+    const int64_t k[3] = {c->k_stride_page, c->k_stride_head, c->k_stride_slot};
+    const int64_t v[3] = {c->v_stride_page, c->v_stride_head, c->v_stride_slot};
+    if (!aligned16(c->k) || !aligned16(c->v) || !make_tensor(c->k, k, *c, cache_es, 16, out.k) ||
+        !make_tensor(c->v, v, *c, cache_es, 16, out.v))
         return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k and v of the cache and their strides must be multiples "
-                                                        "of 16 bytes", op);
+                                                        "of 16 bytes, and strides within 0 .. 64 GB", op);
+    const int64_t ks[3] = {c->ks_stride_page, c->ks_stride_head, c->ks_stride_slot};
+    const int64_t vs[3] = {c->vs_stride_page, c->vs_stride_head, c->vs_stride_slot};
+    if (e4m3 && (!make_tensor(c->k_scale, ks, *c, 4, 4, out.ks) || !make_tensor(c->v_scale, vs, *c, 4, 4, out.vs)))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: strides of the scales must be within 0 .. 16 GB", op);
     out.num_pages = static_cast<int>(c->num_pages);
     out.kv_heads = static_cast<int>(c->kv_heads);
     out.head_dim = static_cast<int>(c->head_dim);
@@ -147,6 +163,29 @@ struct Row8 {
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = make_uint4(0, 0, 0, 0);
     }
+    // The largest finite magnitude, or 0. Magnitudes of 16-bit types compare as
+    // integers, two at a time; infinities and NaN, which are the largest of
+    // them, are looked for only where there are any.
+    __device__ __forceinline__ float largest() const {
+        if constexpr (sizeof(T) == 2) {
+            constexpr uint32_t INF = std::is_same_v<T, __half> ? 0x7c00 : 0x7f80;
+            const uint32_t m = 0x7fff7fffu;
+            uint32_t t = __vmaxu2(__vmaxu2(w[0].x & m, w[0].y & m), __vmaxu2(w[0].z & m, w[0].w & m));
+            t = max(t >> 16, t & 0xffffu);
+            if (t < INF) {
+                const uint16_t bits = static_cast<uint16_t>(t);
+                return to_f32(*reinterpret_cast<const T*>(&bits));
+            }
+        }
+        float x[8], top = 0.0f;
+        get(x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = fabsf(x[i]);
+            if (a < INFINITY) top = fmaxf(top, a);  // false for NaN too
+        }
+        return top;
+    }
 };
 
 constexpr int kThreads = 256;
@@ -202,13 +241,7 @@ __device__ __forceinline__ void store_row(const Row8<T>& row, const PagedTensor&
     if constexpr (QUANT) {
         float x[8];
         row.get(x);
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float m = fabsf(x[i]);
-            if (m < INFINITY) top = fmaxf(top, m);  // false for NaN too
-        }
-        if (!active) top = 0.0f;
+        float top = row.largest();  // idle lanes hold zeros
         for (int off = 1 << lanes_log2 >> 1; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         const int e = top > 0.0f ? scale_exponent(top) : 0;
         const float inv = exp2_int(-e);
@@ -216,13 +249,12 @@ __device__ __forceinline__ void store_row(const Row8<T>& row, const PagedTensor&
         for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], inv);  // exact, or below half of e4m3's least step
         if (store) {
             if (active) {
-                uint8_t* p = static_cast<uint8_t*>(to.p) + to.offset(page, h, slot) + lane_of_row * 8;
-                *reinterpret_cast<uint2*>(p) = to_e4m3(x);
+                *reinterpret_cast<uint2*>(to.row(page, h, slot) + lane_of_row * 8) = to_e4m3(x);
             }
-            if (lane_of_row == 0) static_cast<float*>(scale.p)[scale.offset(page, h, slot)] = exp2_int(e);
+            if (lane_of_row == 0) *scale.scale(page, h, slot) = exp2_int(e);
         }
     } else {
-        if (store && active) row.store(to.p, to.offset(page, h, slot) + lane_of_row * 8);
+        if (store && active) row.store(to.row(page, h, slot), lane_of_row * 8);
     }
 }
 
@@ -367,11 +399,11 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
         v[i].zero();
         ks[i] = vs[i] = 0.0f;
         if (page[i] >= 0) {
-            k[i].load(a.cache.k.p, a.cache.k.offset(page[i], h[i], slot[i]) + c * EACH);
-            v[i].load(a.cache.v.p, a.cache.v.offset(page[i], h[i], slot[i]) + c * EACH);
+            k[i].load(a.cache.k.row(page[i], h[i], slot[i]), c * EACH);
+            v[i].load(a.cache.v.row(page[i], h[i], slot[i]), c * EACH);
             if constexpr (QUANT) {
-                ks[i] = static_cast<const float*>(a.cache.ks.p)[a.cache.ks.offset(page[i], h[i], slot[i])];
-                vs[i] = static_cast<const float*>(a.cache.vs.p)[a.cache.vs.offset(page[i], h[i], slot[i])];
+                ks[i] = *a.cache.ks.scale(page[i], h[i], slot[i]);
+                vs[i] = *a.cache.vs.scale(page[i], h[i], slot[i]);
             }
         }
     }

@@ -14,14 +14,23 @@
 
 namespace ako_b200 {
 
-// One of a cache's tensors: element strides over pages, heads and slots.
+// One of a cache's tensors, with strides over pages, heads and slots in units
+// of 16 bytes (keys and values) or of a float (scales). 32-bit strides make an
+// offset three multiply-adds; they reach 64 GB.
 struct PagedTensor {
     void* p;
-    int64_t page, head, slot;
+    uint32_t page, head, slot;
 
-    __device__ __forceinline__ int64_t offset(int pg, int h, int s) const {
-        return pg * page + h * head + s * slot;
+    __device__ __forceinline__ uint64_t offset(int pg, int h, int s) const {
+        return static_cast<uint64_t>(page) * static_cast<uint32_t>(pg) +
+               static_cast<uint64_t>(head) * static_cast<uint32_t>(h) +
+               static_cast<uint64_t>(slot) * static_cast<uint32_t>(s);
     }
+    // Of a row of keys or values.
+    __device__ __forceinline__ uint8_t* row(int pg, int h, int s) const {
+        return static_cast<uint8_t*>(p) + offset(pg, h, s) * 16;
+    }
+    __device__ __forceinline__ float* scale(int pg, int h, int s) const { return static_cast<float*>(p) + offset(pg, h, s); }
 };
 
 struct PagedCache {

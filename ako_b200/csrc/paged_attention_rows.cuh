@@ -193,9 +193,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                         const PagedTensor& t = kv == 0 ? a.cache.k : a.cache.v;
                         const int c = lane % CHUNKS, row = lane / CHUNKS;
                         const int first = slot - (lane & 15);  // the first key's slot
-                        const uint8_t* from = static_cast<const uint8_t*>(t.p) +
-                                              (t.offset(page, it.h, first + row) * BYTES + c * 16);
-                        const int64_t step = t.slot * (TAKEN * BYTES);
+                        const uint8_t* from = t.row(page, it.h, first + row) + c * 16;
+                        const uint64_t step = static_cast<uint64_t>(t.slot) * (TAKEN * 16);
                         const bool real = c * 16 < dim * BYTES;
 #pragma unroll
                         for (int i = 0; i < kWarpKeys / TAKEN; ++i) {
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                         }
                     }
                 } else {
-                    const int64_t off = page >= 0 ? mine.offset(page, it.h, slot) : -1;
+                    const int64_t off = page >= 0 ? static_cast<int64_t>(mine.offset(page, it.h, slot)) : -1;
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         const uint8_t* base = static_cast<const uint8_t*>(kv == 0 ? a.cache.k.p : a.cache.v.p);
@@ -218,15 +217,14 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                             const int sc =
                                 kv == 0 ? swizzled<QUANT, DPAD, true>(row, c) : swizzled<QUANT, DPAD, false>(row, c);
                             cp_async16_or_zero(to + (kv * kWarpKeys + row) * ROWB + sc * 16,
-                                               real ? base + o * BYTES + c * 16 : base, real);
+                                               real ? base + o * 16 + c * 16 : base, real);
                         }
                     }
                 }
                 if constexpr (QUANT) {
                     const PagedTensor& st = lane < 16 ? a.cache.ks : a.cache.vs;
-                    const float* p = static_cast<const float*>(st.p);
                     cp_async4_or_zero(to + 2 * kWarpKeys * ROWB + lane * 4,
-                                      page >= 0 ? p + st.offset(page, it.h, slot) : p, page >= 0);
+                                      page >= 0 ? st.scale(page, it.h, slot) : static_cast<float*>(st.p), page >= 0);
                 }
                 if (lane == 0)
                     *reinterpret_cast<volatile uint32_t*>(ring + (stage + 1) * Shape::kStageBytes - 16) = there;

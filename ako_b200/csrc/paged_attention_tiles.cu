@@ -28,7 +28,7 @@ bool make_map(const PagedTensor& t, const PagedCache& c, bool half, int box, CUt
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
                                 static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.num_pages)};
     // the stride of an axis of one element plays no part, but has to be a valid one
-    auto bytes = [&](int64_t stride, int n) { return static_cast<cuuint64_t>(n > 1 ? stride * 2 : 256); };
+    auto bytes = [&](uint32_t stride, int n) { return n > 1 ? static_cast<cuuint64_t>(stride) * 16 : 256; };
     const cuuint64_t strides[3] = {bytes(t.slot, c.page_size), bytes(t.head, c.kv_heads), bytes(t.page, c.num_pages)};
     const cuuint32_t boxes[4] = {64, static_cast<cuuint32_t>(box), 1, 1}, steps[4] = {1, 1, 1, 1};
     return encode(&map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.p, dims, strides,

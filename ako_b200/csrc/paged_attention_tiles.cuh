@@ -131,14 +131,14 @@ __device__ __forceinline__ void add_odd_values(const AttnArgs& a, const Item& it
             if (!sees_key(a, pos, key)) continue;
             const int page = page_of(a.seqs, a.cache, it.b, key, slot);
             if (page < 0) continue;
-            const int64_t at = a.cache.v.offset(page, it.h, slot);
+            const uint8_t* const row = a.cache.v.row(page, it.h, slot);
             for (int d = 0; d < a.cache.head_dim; ++d) {
                 float x;
                 if constexpr (QUANT) {
-                    const uint8_t e = static_cast<const uint8_t*>(a.cache.v.p)[at + d];
+                    const uint8_t e = row[d];
                     x = (e & 0x7f) == 0x7f ? NAN : 0.0f;
                 } else {
-                    x = to_f32(static_cast<const T*>(a.cache.v.p)[at + d]);
+                    x = to_f32(reinterpret_cast<const T*>(row)[d]);
                 }
                 if (!isfinite(x)) out[d] = from_f32<O>(to_f32(out[d]) + x);
             }
@@ -185,7 +185,7 @@ struct TileLoader {
     };
     // Where its row is.
     struct Rows {
-        int64_t k, v;  // offsets, or -1
+        int64_t k, v;  // offsets in 16 bytes, or -1
         float ks, vs;
         bool whole;
     };
@@ -221,11 +221,11 @@ struct TileLoader {
     __device__ __forceinline__ Rows find(const Place& p) const {
         Rows r{-1, -1, 0.0f, 1.0f, p.whole};
         if (there(p)) {
-            r.k = a.cache.k.offset(p.page, p.h, p.slot);
-            r.v = a.cache.v.offset(p.page, p.h, p.slot);
+            r.k = static_cast<int64_t>(a.cache.k.offset(p.page, p.h, p.slot));
+            r.v = static_cast<int64_t>(a.cache.v.offset(p.page, p.h, p.slot));
             if constexpr (QUANT) {
-                r.ks = static_cast<const float*>(a.cache.ks.p)[a.cache.ks.offset(p.page, p.h, p.slot)];
-                r.vs = static_cast<const float*>(a.cache.vs.p)[a.cache.vs.offset(p.page, p.h, p.slot)];
+                r.ks = *a.cache.ks.scale(p.page, p.h, p.slot);
+                r.vs = *a.cache.vs.scale(p.page, p.h, p.slot);
             }
         }
         return r;
@@ -241,7 +241,7 @@ struct TileLoader {
 
     // 16-bit caches: copies straight into the tile.
     __device__ __forceinline__ void copy(const PagedTensor& from, const Place& p, uint32_t tile, int more) const {
-        const int64_t offset = there(p) ? from.offset(p.page, p.h, p.slot) : -1;
+        const int64_t offset = there(p) ? static_cast<int64_t>(from.offset(p.page, p.h, p.slot)) : -1;
         // The places first: the copies' order is fixed, and each would wait for its own.
         int64_t o[EACH];
 #pragma unroll
@@ -250,7 +250,7 @@ struct TileLoader {
         for (int i = 0; i < EACH; ++i) {
             const bool there = o[i] >= 0 && real;
             cp_async16_or_zero(tile + place(rows0 + more + row0 + i * ROWS, chunk),
-                               static_cast<const uint8_t*>(from.p) + (there ? (o[i] + chunk * 8) * 2 : 0), there);
+                               static_cast<const uint8_t*>(from.p) + (there ? (o[i] + chunk) * 16 : 0), there);
         }
     }
 
@@ -275,7 +275,7 @@ struct TileLoader {
         for (int i = 0; i < EACH; ++i) {
             const int64_t o = __shfl_sync(0xffffffffu, offset, row0 + i * ROWS);
             v[i] = make_uint4(0, 0, 0, 0);
-            if (o >= 0 && real) v[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + o + chunk * 16);
+            if (o >= 0 && real) v[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + (o + chunk) * 16);
         }
     }
 
