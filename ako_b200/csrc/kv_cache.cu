@@ -16,23 +16,19 @@ namespace {
 
 bool multiple16(int64_t stride, int64_t extent, int es) { return extent <= 1 || ((stride * es) & 15) == 0; }
 
-// A tensor's view, strides in units of `unit` bytes (those of axes of one
-// element play no part); false if a stride does not fit.
-bool make_tensor(void* p, const int64_t (&strides)[3], const ako_b200_paged_kv& c, int es, int unit, PagedTensor& out) {
-    const int64_t extents[3] = {c.num_pages, c.kv_heads, c.page_size};
-    uint32_t units[3];
-    for (int i = 0; i < 3; ++i) {
-        if (extents[i] <= 1) {
-            units[i] = 0;
-            continue;
-        }
-        if (strides[i] < 0 || strides[i] > INT64_MAX / 16 || strides[i] * es % unit != 0 ||
-            strides[i] * es / unit > UINT32_MAX)
-            return false;
-        units[i] = static_cast<uint32_t>(strides[i] * es / unit);
-    }
-    out = PagedTensor{p, units[0], units[1], units[2]};
+// A stride of `stride` elements in units of `unit` bytes; false if it is none that fits.
+bool stride_units(int64_t stride, int es, int unit, uint32_t& out) {
+    if (stride < 0 || stride > INT64_MAX / 16 || stride * es % unit != 0 || stride * es / unit > UINT32_MAX) return false;
+    out = static_cast<uint32_t>(stride * es / unit);
     return true;
+}
+
+// A cache tensor's view; strides of axes of one element play no part.
+bool make_tensor(void* p, const int64_t (&strides)[3], const ako_b200_paged_kv& c, int es, int unit, PagedTensor& out) {
+    out.p = p;
+    return stride_units(c.num_pages > 1 ? strides[0] : 0, es, unit, out.page) &&
+           stride_units(c.kv_heads > 1 ? strides[1] : 0, es, unit, out.head) &&
+           stride_units(c.page_size > 1 ? strides[2] : 0, es, unit, out.slot);
 }
 
 }  // namespace
@@ -109,15 +105,6 @@ int make_seqs(const char* op, const ako_b200_paged_batch* b, const PagedCache& c
 namespace {
 
 // ------------------------------------------------------------------ e4m3
-// Eight fp32 values as e4m3, to nearest even, saturating (NaN stays NaN).
-__device__ __forceinline__ uint2 to_e4m3(const float (&x)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-    return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-}
-
 __device__ __forceinline__ float2 from_e4m3(uint32_t pair) {
     return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3)));
 }
@@ -163,6 +150,29 @@ struct Row8 {
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = make_uint4(0, 0, 0, 0);
     }
+    // Times 2^e, as e4m3: to nearest even, saturating. The product is exact, or
+    // below 2^-14 and so rounds to zero either way.
+    __device__ __forceinline__ uint2 scaled_e4m3(int e) const {
+        uint32_t y[4];
+        if (std::is_same_v<T, __half> && e >= -14 && e <= 15) {
+            const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+            const __half2 f = __half2half2(__float2half_rn(exp2_int(e)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&u[i]), f);
+                y[i] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(p), __NV_SATFINITE, __NV_E4M3);
+            }
+        } else {
+            const float f = exp2_int(e);
+            float x[8];
+            get(x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                y[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[2 * i], f), __fmul_rn(x[2 * i + 1], f)),
+                                                __NV_SATFINITE, __NV_E4M3);
+        }
+        return make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
+    }
     // The largest finite magnitude, or 0. Magnitudes of 16-bit types compare as
     // integers, two at a time; infinities and NaN, which are the largest of
     // them, are looked for only where there are any.
@@ -198,16 +208,20 @@ int lanes_log2(int head_dim, int each) {
     return l;
 }
 
-// Rows per thread: the most that still gives every SM `ctas` CTAs.
-int rows_per_thread(int64_t rows, int rows_per_pass, int most, int ctas) {
-    const int64_t passes = (rows + rows_per_pass - 1) / rows_per_pass;
-    return passes >= static_cast<int64_t>(most) * ctas * sm_count() ? most : 1;
-}
-
 // ------------------------------------------------------------------- write
+// Rows of new tokens: strides over sequences, tokens and heads, in 16 bytes.
+struct NewRows {
+    const void* p;
+    uint32_t b, s, h;
+
+    __device__ __forceinline__ const uint8_t* row(uint32_t bi, uint32_t si, uint32_t hi) const {
+        return static_cast<const uint8_t*>(p) +
+               (static_cast<uint64_t>(b) * bi + static_cast<uint64_t>(s) * si + static_cast<uint64_t>(h) * hi) * 16;
+    }
+};
+
 struct WriteArgs {
-    const void *k, *v;
-    int64_t kb, ks, kh, vb, vs, vh;
+    NewRows k, v;
     PagedCache cache;
     PagedSeqs seqs;
     FastDiv heads, q_len;
@@ -239,18 +253,11 @@ __device__ __forceinline__ void store_row(const Row8<T>& row, const PagedTensor&
                                           bool store, int page, int h, int slot, int lane_of_row, int lanes_log2,
                                           bool active) {
     if constexpr (QUANT) {
-        float x[8];
-        row.get(x);
         float top = row.largest();  // idle lanes hold zeros
         for (int off = 1 << lanes_log2 >> 1; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         const int e = top > 0.0f ? scale_exponent(top) : 0;
-        const float inv = exp2_int(-e);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], inv);  // exact, or below half of e4m3's least step
         if (store) {
-            if (active) {
-                *reinterpret_cast<uint2*>(to.row(page, h, slot) + lane_of_row * 8) = to_e4m3(x);
-            }
+            if (active) *reinterpret_cast<uint2*>(to.row(page, h, slot) + lane_of_row * 8) = row.scaled_e4m3(-e);
             if (lane_of_row == 0) *scale.scale(page, h, slot) = exp2_int(e);
         }
     } else {
@@ -262,7 +269,9 @@ __device__ __forceinline__ void store_row(const Row8<T>& row, const PagedTensor&
 // 2^lanes_log2 lanes share such a row (those behind head_dim idle), and a
 // thread takes ROWS rows, so that 2 * ROWS loads are under way while it finds
 // their pages.
-// Bound: HBM for prompts, the chain cu_seqlens -> length -> page for a step.
+// Bound: HBM for prompts as they are (82.6 MB in 15.3 us, 5.4 TB/s), the
+// issue of instructions for prompts that are quantised, the chain
+// cu_seqlens -> length -> page for a step.
 template <typename T, bool QUANT, int ROWS>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
     pdl_enter();
@@ -271,42 +280,41 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
     const uint32_t row0 = blockIdx.x * (pass * ROWS) + (threadIdx.x >> a.lanes_log2);
     const bool active = c * 8 < a.cache.head_dim;
     Row8<T> k[ROWS], v[ROWS];
-    int t[ROWS], h[ROWS];
+    uint32_t t[ROWS], h[ROWS], b[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         // rows behind the last repeat it and are not stored
         const uint32_t row = min(row0 + i * pass, a.rows - 1);
-        t[i] = static_cast<int>(a.heads.div(row));
-        h[i] = static_cast<int>(row - t[i] * a.heads.d);
-        int64_t b = 0, s = t[i];
+        t[i] = a.heads.div(row);
+        h[i] = row - t[i] * a.heads.d;
+        b[i] = 0;
+        uint32_t s = t[i];
         if (a.seqs.cu == nullptr) {
-            b = a.q_len.div(t[i]);
-            s -= b * a.q_len.d;
+            b[i] = a.q_len.div(t[i]);
+            s -= b[i] * a.q_len.d;
         }
+        k[i].zero();
+        v[i].zero();
         if (active) {
-            k[i].load(a.k, b * a.kb + s * a.ks + h[i] * a.kh + c * 8);
-            v[i].load(a.v, b * a.vb + s * a.vs + h[i] * a.vh + c * 8);
-        } else {
-            k[i].zero();
-            v[i].zero();
+            k[i].load(a.k.row(b[i], s, h[i]), c * 8);
+            v[i].load(a.v.row(b[i], s, h[i]), c * 8);
         }
     }
-    int b = a.seqs.cu == nullptr ? 0 : find_sequence(a.seqs.cu, a.seqs.batch, t[0]);
+    if (a.seqs.cu != nullptr) b[0] = find_sequence(a.seqs.cu, a.seqs.batch, static_cast<int>(t[0]));
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        if (a.seqs.cu == nullptr) {
-            b = static_cast<int>(a.q_len.div(t[i]));
-        } else {
-            while (b + 1 < a.seqs.batch && a.seqs.cu[b + 1] <= t[i]) ++b;
+        if (i > 0 && a.seqs.cu != nullptr) {
+            b[i] = b[i - 1];
+            while (static_cast<int>(b[i]) + 1 < a.seqs.batch && a.seqs.cu[b[i] + 1] <= static_cast<int>(t[i])) ++b[i];
         }
         int first, n;
-        new_tokens(a.seqs, b, first, n);
-        const int at = t[i] - first;
-        const int pos = cached_tokens(a.seqs, b) - n + at;
-        bool store = row0 + i * pass < a.rows && at >= 0 && at < n && pos >= 0;
+        new_tokens(a.seqs, static_cast<int>(b[i]), first, n);
+        const int at = static_cast<int>(t[i]) - first;
+        const int pos = cached_tokens(a.seqs, static_cast<int>(b[i])) - n + at;
+        const bool there = row0 + i * pass < a.rows && at >= 0 && at < n && pos >= 0;
         int slot = 0;
-        const int page = store ? page_of(a.seqs, a.cache, b, pos, slot) : -1;
-        store = page >= 0;
+        const int page = there ? page_of(a.seqs, a.cache, static_cast<int>(b[i]), pos, slot) : -1;
+        const bool store = page >= 0;
         store_row<T, QUANT>(k[i], a.cache.k, a.cache.ks, store, page, h[i], slot, c, a.lanes_log2, active);
         store_row<T, QUANT>(v[i], a.cache.v, a.cache.vs, store, page, h[i], slot, c, a.lanes_log2, active);
     }
@@ -315,15 +323,15 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
 template <typename T>
 int launch_write(WriteArgs& a, bool quant, cudaStream_t st) {
     a.lanes_log2 = lanes_log2(a.cache.head_dim, 8);
-    const int pass = kThreads >> a.lanes_log2;
-    const int each = rows_per_thread(a.rows, pass, 4, 4);
-    const dim3 grid(static_cast<unsigned>((int64_t{a.rows} + int64_t{pass} * each - 1) / (int64_t{pass} * each)));
+    const int64_t pass = kThreads >> a.lanes_log2;
     const char* name = "kv_cache_write";
-    if (quant)
-        return each == 4 ? launch_ex(kv_write_kernel<T, true, 4>, grid, dim3(kThreads), 0, 1, st, a, name)
-                         : launch_ex(kv_write_kernel<T, true, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
-    return each == 4 ? launch_ex(kv_write_kernel<T, false, 4>, grid, dim3(kThreads), 0, 1, st, a, name)
-                     : launch_ex(kv_write_kernel<T, false, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+    // Two rows to a thread where that leaves every SM four CTAs, for quantised rows, whose chain of
+    // instructions is long (216 MB: 57 us against 63); as they are, one (82.6 MB: 15.3 us against 15.8).
+    const int64_t each = quant && a.rows >= pass * 8 * sm_count() ? 2 : 1;
+    const dim3 grid(static_cast<unsigned>((a.rows + pass * each - 1) / (pass * each)));
+    if (each == 2) return launch_ex(kv_write_kernel<T, true, 2>, grid, dim3(kThreads), 0, 1, st, a, name);
+    if (quant) return launch_ex(kv_write_kernel<T, true, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+    return launch_ex(kv_write_kernel<T, false, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
 }
 
 // -------------------------------------------------------------------- read
@@ -366,74 +374,65 @@ struct Row16Q {
 };
 
 // A lane moves 16 bytes of a row of the cache (a position's keys in one head)
-// and the same of its values, for ROWS rows. Rows run over positions first,
-// along a page and along the output.
-template <typename T, bool QUANT, int ROWS>
+// and the same of its values. Rows run over positions first, along a page and
+// along the output. One row to a thread: with two the same bytes are under way
+// in half the CTAs, which measured 144 us against 131 for 744 MB (e4m3 to bf16).
+template <typename T, bool QUANT>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
     pdl_enter();
     using Held = std::conditional_t<QUANT, Row16Q, Row8<T>>;
     constexpr int EACH = QUANT ? 16 : 8;
     const int c = static_cast<int>(threadIdx.x) & ((1 << a.lanes_log2) - 1);
-    if (c * EACH >= a.cache.head_dim) return;
-    const uint32_t pass = kThreads >> a.lanes_log2;
-    const uint32_t row0 = blockIdx.x * (pass * ROWS) + (threadIdx.x >> a.lanes_log2);
-    Held k[ROWS], v[ROWS];
-    float ks[ROWS], vs[ROWS];
-    uint32_t j[ROWS];
-    int h[ROWS], b[ROWS], page[ROWS], slot[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const uint32_t row = min(row0 + i * pass, a.rows - 1);
-        const uint32_t bh = a.length.div(row);
-        j[i] = row - bh * a.length.d;
-        b[i] = static_cast<int>(a.heads.div(bh));
-        h[i] = static_cast<int>(bh - b[i] * a.heads.d);
-        const int64_t pos = a.start + j[i];
-        page[i] = -1;
-        slot[i] = 0;
-        if (pos < cached_tokens(a.seqs, b[i])) page[i] = page_of(a.seqs, a.cache, b[i], static_cast<int>(pos), slot[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        k[i].zero();
-        v[i].zero();
-        ks[i] = vs[i] = 0.0f;
-        if (page[i] >= 0) {
-            k[i].load(a.cache.k.row(page[i], h[i], slot[i]), c * EACH);
-            v[i].load(a.cache.v.row(page[i], h[i], slot[i]), c * EACH);
-            if constexpr (QUANT) {
-                ks[i] = *a.cache.ks.scale(page[i], h[i], slot[i]);
-                vs[i] = *a.cache.vs.scale(page[i], h[i], slot[i]);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        if (row0 + i * pass >= a.rows) return;
-        const int64_t ko = b[i] * a.kb + h[i] * a.kh + j[i] * a.ks + c * EACH;
-        const int64_t vo = b[i] * a.vb + h[i] * a.vh + j[i] * a.vs + c * EACH;
+    const uint32_t row = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+    if (c * EACH >= a.cache.head_dim || row >= a.rows) return;
+    const uint32_t bh = a.length.div(row);
+    const uint32_t j = row - bh * a.length.d;
+    const int b = static_cast<int>(a.heads.div(bh));
+    const int h = static_cast<int>(bh - b * a.heads.d);
+    const int64_t pos = a.start + j;
+    int page = -1, slot = 0;
+    if (pos < cached_tokens(a.seqs, b)) page = page_of(a.seqs, a.cache, b, static_cast<int>(pos), slot);
+    Held k, v;
+    [[maybe_unused]] float ks = 0.0f, vs = 0.0f;
+    k.zero();
+    v.zero();
+    if (page >= 0) {
+        k.load(a.cache.k.row(page, h, slot), c * EACH);
+        v.load(a.cache.v.row(page, h, slot), c * EACH);
         if constexpr (QUANT) {
-            k[i].template store<T>(a.k, ko, ks[i]);
-            v[i].template store<T>(a.v, vo, vs[i]);
-        } else {
-            k[i].store(a.k, ko);
-            v[i].store(a.v, vo);
+            ks = *a.cache.ks.scale(page, h, slot);
+            vs = *a.cache.vs.scale(page, h, slot);
         }
+    }
+    const int64_t ko = b * a.kb + h * a.kh + j * a.ks + c * EACH;
+    const int64_t vo = b * a.vb + h * a.vh + j * a.vs + c * EACH;
+    if constexpr (QUANT) {
+        k.template store<T>(a.k, ko, ks);
+        v.template store<T>(a.v, vo, vs);
+    } else {
+        k.store(a.k, ko);
+        v.store(a.v, vo);
     }
 }
 
 template <typename T>
 int launch_read(ReadArgs& a, bool quant, cudaStream_t st) {
     a.lanes_log2 = lanes_log2(a.cache.head_dim, quant ? 16 : 8);
-    const int pass = kThreads >> a.lanes_log2;
-    const int each = rows_per_thread(a.rows, pass, 2, 8);
-    const dim3 grid(static_cast<unsigned>((int64_t{a.rows} + int64_t{pass} * each - 1) / (int64_t{pass} * each)));
+    const int64_t pass = kThreads >> a.lanes_log2;
+    const dim3 grid(static_cast<unsigned>((int64_t{a.rows} + pass - 1) / pass));
     const char* name = "kv_cache_read";
-    if (quant)
-        return each == 2 ? launch_ex(kv_read_kernel<T, true, 2>, grid, dim3(kThreads), 0, 1, st, a, name)
-                         : launch_ex(kv_read_kernel<T, true, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
-    return each == 2 ? launch_ex(kv_read_kernel<T, false, 2>, grid, dim3(kThreads), 0, 1, st, a, name)
-                     : launch_ex(kv_read_kernel<T, false, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+    return quant ? launch_ex(kv_read_kernel<T, true>, grid, dim3(kThreads), 0, 1, st, a, name)
+                 : launch_ex(kv_read_kernel<T, false>, grid, dim3(kThreads), 0, 1, st, a, name);
+}
+
+bool make_rows(const void* p, int64_t sb, int64_t nb, int64_t ss, int64_t ns, int64_t sh, int64_t nh, int es,
+               NewRows& out) {
+    const int64_t strides[3] = {nb > 1 ? sb : 0, ns > 1 ? ss : 0, nh > 1 ? sh : 0};
+    uint32_t units[3];
+    for (int i = 0; i < 3; ++i)
+        if (!stride_units(strides[i], es, 16, units[i])) return false;
+    out = NewRows{p, units[0], units[1], units[2]};
+    return aligned16(p);
 }
 
 // Pointer and the strides of axes longer than one are multiples of 16 bytes.
@@ -466,20 +465,14 @@ extern "C" int ako_b200_kv_cache_write(const void* k, int64_t k_stride_b, int64_
     const bool uniform = a.seqs.cu == nullptr;
     const int64_t nb = uniform ? a.seqs.batch : 1, ns = uniform ? q_len : tokens;
     const int in = dtype_size(dtype);
-    if (!rows16(k, k_stride_b, nb, k_stride_s, ns, k_stride_h, a.cache.kv_heads, in) ||
-        !rows16(v, v_stride_b, nb, v_stride_s, ns, v_stride_h, a.cache.kv_heads, in))
-        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k, v and their strides must be multiples of 16 bytes", op);
-    a.k = k;
-    a.v = v;
-    a.kb = k_stride_b;
-    a.ks = k_stride_s;
-    a.kh = k_stride_h;
-    a.vb = v_stride_b;
-    a.vs = v_stride_s;
-    a.vh = v_stride_h;
+    const bool fit = make_rows(k, k_stride_b, nb, k_stride_s, ns, k_stride_h, a.cache.kv_heads, in, a.k) &&
+                     make_rows(v, v_stride_b, nb, v_stride_s, ns, v_stride_h, a.cache.kv_heads, in, a.v);
+    if (!fit)
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT,
+                         "%s: k, v and their strides must be multiples of 16 bytes, and strides within 0 .. 64 GB", op);
     a.heads = FastDiv::make(static_cast<uint32_t>(a.cache.kv_heads));
-    a.q_len = FastDiv::make(static_cast<uint32_t>(uniform ? q_len : 1));
     a.rows = static_cast<uint32_t>(tokens * a.cache.kv_heads);
+    a.q_len = FastDiv::make(static_cast<uint32_t>(uniform ? q_len : 1));
     const bool quant = cache->dtype == AKO_B200_E4M3;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
