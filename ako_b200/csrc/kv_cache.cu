@@ -248,90 +248,80 @@ __device__ __forceinline__ int find_sequence(const int* cu, int batch, int t) {
     return lo;
 }
 
-template <typename T, bool QUANT>
-__device__ __forceinline__ void store_row(const Row8<T>& row, const PagedTensor& to, const PagedTensor& scale,
-                                          bool store, int page, int h, int slot, int lane_of_row, int lanes_log2,
-                                          bool active) {
-    if constexpr (QUANT) {
-        float top = row.largest();  // idle lanes hold zeros
-        for (int off = 1 << lanes_log2 >> 1; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const int e = top > 0.0f ? scale_exponent(top) : 0;
-        if (store) {
-            if (active) *reinterpret_cast<uint2*>(to.row(page, h, slot) + lane_of_row * 8) = row.scaled_e4m3(-e);
-            if (lane_of_row == 0) *scale.scale(page, h, slot) = exp2_int(e);
-        }
-    } else {
-        if (store && active) row.store(to.row(page, h, slot), lane_of_row * 8);
+// Quantises the row that 2^lanes_log2 lanes hold sixteen values each of, and stores it.
+template <typename T>
+__device__ __forceinline__ void store_quantised(const Row8<T> (&x)[2], const PagedTensor& to, const PagedTensor& scale,
+                                                bool store, int page, int h, int slot, int lane_of_row, int lanes_log2,
+                                                bool active) {
+    float top = fmaxf(x[0].largest(), x[1].largest());  // idle lanes hold zeros
+    for (int off = 1 << lanes_log2 >> 1; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const int e = top > 0.0f ? scale_exponent(top) : 0;
+    if (!store) return;
+    if (active) {
+        const uint2 lo = x[0].scaled_e4m3(-e), hi = x[1].scaled_e4m3(-e);
+        *reinterpret_cast<uint4*>(to.row(page, h, slot) + lane_of_row * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
+    if (lane_of_row == 0) *scale.scale(page, h, slot) = exp2_int(e);
 }
 
-// A lane moves eight values of a token's keys and of its values in one head;
-// 2^lanes_log2 lanes share such a row (those behind head_dim idle), and a
-// thread takes ROWS rows, so that 2 * ROWS loads are under way while it finds
-// their pages.
-// Bound: HBM for prompts as they are (82.6 MB in 15.3 us, 5.4 TB/s), the
-// issue of instructions for prompts that are quantised, the chain
+// A lane moves eight values, sixteen where they are quantised, of a token's
+// keys and of its values in one head; 2^lanes_log2 lanes share such a row
+// (those behind head_dim idle). The loads are under way while the thread finds
+// the row's page.
+// Bound: HBM for prompts as they are (82.6 MB in 15.3 us, 5.4 TB/s); for
+// quantised ones the issue of instructions, of which sixteen values to a lane
+// take fewer than eight (216 MB of fp16: 38 us against 54); the chain
 // cu_seqlens -> length -> page for a step.
-template <typename T, bool QUANT, int ROWS>
+template <typename T, bool QUANT>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
     pdl_enter();
+    constexpr int PARTS = QUANT ? 2 : 1;
     const int c = static_cast<int>(threadIdx.x) & ((1 << a.lanes_log2) - 1);
-    const uint32_t pass = kThreads >> a.lanes_log2;
-    const uint32_t row0 = blockIdx.x * (pass * ROWS) + (threadIdx.x >> a.lanes_log2);
-    const bool active = c * 8 < a.cache.head_dim;
-    Row8<T> k[ROWS], v[ROWS];
-    uint32_t t[ROWS], h[ROWS], b[ROWS];
+    const uint32_t at_row = blockIdx.x * (kThreads >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+    const bool active = c * PARTS * 8 < a.cache.head_dim;
+    // rows behind the last repeat it and are not stored
+    const uint32_t row = min(at_row, a.rows - 1);
+    const uint32_t t = a.heads.div(row);
+    const int h = static_cast<int>(row - t * a.heads.d);
+    uint32_t b = 0, s = t;
+    if (a.seqs.cu == nullptr) {
+        b = a.q_len.div(t);
+        s -= b * a.q_len.d;
+    }
+    Row8<T> k[PARTS], v[PARTS];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        // rows behind the last repeat it and are not stored
-        const uint32_t row = min(row0 + i * pass, a.rows - 1);
-        t[i] = a.heads.div(row);
-        h[i] = row - t[i] * a.heads.d;
-        b[i] = 0;
-        uint32_t s = t[i];
-        if (a.seqs.cu == nullptr) {
-            b[i] = a.q_len.div(t[i]);
-            s -= b[i] * a.q_len.d;
-        }
+    for (int i = 0; i < PARTS; ++i) {
         k[i].zero();
         v[i].zero();
         if (active) {
-            k[i].load(a.k.row(b[i], s, h[i]), c * 8);
-            v[i].load(a.v.row(b[i], s, h[i]), c * 8);
+            k[i].load(a.k.row(b, s, h), (c * PARTS + i) * 8);
+            v[i].load(a.v.row(b, s, h), (c * PARTS + i) * 8);
         }
     }
-    if (a.seqs.cu != nullptr) b[0] = find_sequence(a.seqs.cu, a.seqs.batch, static_cast<int>(t[0]));
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        if (i > 0 && a.seqs.cu != nullptr) {
-            b[i] = b[i - 1];
-            while (static_cast<int>(b[i]) + 1 < a.seqs.batch && a.seqs.cu[b[i] + 1] <= static_cast<int>(t[i])) ++b[i];
-        }
-        int first, n;
-        new_tokens(a.seqs, static_cast<int>(b[i]), first, n);
-        const int at = static_cast<int>(t[i]) - first;
-        const int pos = cached_tokens(a.seqs, static_cast<int>(b[i])) - n + at;
-        const bool there = row0 + i * pass < a.rows && at >= 0 && at < n && pos >= 0;
-        int slot = 0;
-        const int page = there ? page_of(a.seqs, a.cache, static_cast<int>(b[i]), pos, slot) : -1;
-        const bool store = page >= 0;
-        store_row<T, QUANT>(k[i], a.cache.k, a.cache.ks, store, page, h[i], slot, c, a.lanes_log2, active);
-        store_row<T, QUANT>(v[i], a.cache.v, a.cache.vs, store, page, h[i], slot, c, a.lanes_log2, active);
+    if (a.seqs.cu != nullptr) b = find_sequence(a.seqs.cu, a.seqs.batch, static_cast<int>(t));
+    int first, n;
+    new_tokens(a.seqs, static_cast<int>(b), first, n);
+    const int at = static_cast<int>(t) - first;
+    const int pos = cached_tokens(a.seqs, static_cast<int>(b)) - n + at;
+    int slot = 0, page = -1;
+    if (at_row < a.rows && at >= 0 && at < n && pos >= 0) page = page_of(a.seqs, a.cache, static_cast<int>(b), pos, slot);
+    if constexpr (QUANT) {
+        store_quantised(k, a.cache.k, a.cache.ks, page >= 0, page, h, slot, c, a.lanes_log2, active);
+        store_quantised(v, a.cache.v, a.cache.vs, page >= 0, page, h, slot, c, a.lanes_log2, active);
+    } else if (page >= 0 && active) {
+        k[0].store(a.cache.k.row(page, h, slot), c * 8);
+        v[0].store(a.cache.v.row(page, h, slot), c * 8);
     }
 }
 
 template <typename T>
 int launch_write(WriteArgs& a, bool quant, cudaStream_t st) {
-    a.lanes_log2 = lanes_log2(a.cache.head_dim, 8);
+    a.lanes_log2 = lanes_log2(a.cache.head_dim, quant ? 16 : 8);
     const int64_t pass = kThreads >> a.lanes_log2;
     const char* name = "kv_cache_write";
-    // Two rows to a thread where that leaves every SM four CTAs, for quantised rows, whose chain of
-    // instructions is long (216 MB: 57 us against 63); as they are, one (82.6 MB: 15.3 us against 15.8).
-    const int64_t each = quant && a.rows >= pass * 8 * sm_count() ? 2 : 1;
-    const dim3 grid(static_cast<unsigned>((a.rows + pass * each - 1) / (pass * each)));
-    if (each == 2) return launch_ex(kv_write_kernel<T, true, 2>, grid, dim3(kThreads), 0, 1, st, a, name);
-    if (quant) return launch_ex(kv_write_kernel<T, true, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
-    return launch_ex(kv_write_kernel<T, false, 1>, grid, dim3(kThreads), 0, 1, st, a, name);
+    const dim3 grid(static_cast<unsigned>((a.rows + pass - 1) / pass));
+    return quant ? launch_ex(kv_write_kernel<T, true>, grid, dim3(kThreads), 0, 1, st, a, name)
+                 : launch_ex(kv_write_kernel<T, false>, grid, dim3(kThreads), 0, 1, st, a, name);
 }
 
 // -------------------------------------------------------------------- read
