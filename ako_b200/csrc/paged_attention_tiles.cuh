@@ -49,8 +49,8 @@ constexpr int kMetaStages = 8;
 constexpr uint32_t kWaitCycles = 1u << 31;  // of a wait, about a second
 constexpr uint32_t kDrainPolls = 1u << 24;
 // Registers per thread of the softmax, loading and issuing warps. The block is
-// launched with 128 a thread, and 2 * 184 + 96 + 48 = 4 * 128.
-constexpr int kSoftmaxRegs = 184, kLoadRegs = 96, kIssueRegs = 48;
+// launched with 128 a thread, and 2 * 192 + 80 + 48 = 4 * 128.
+constexpr int kSoftmaxRegs = 192, kLoadRegs = 80, kIssueRegs = 48;
 
 struct TilesArgs {
     // The cache's keys and values as (page, head, slot, column) in boxes of `box` slots and 64
@@ -538,33 +538,31 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             typename Loader::Rows rows = load.find(place);
             bool more = step();
             if (more) place = load.look_up(it, key0());
-            uint4 kv[Loader::EACH], vv[Loader::EACH];
-            load.fetch(a.cache.k.p, rows.k, kv);
-            load.fetch(a.cache.v.p, rows.v, vv);
             for (uint32_t n = 0;; ++n) {
                 const int st = n % STAGES;
                 const typename Loader::Rows now = rows;
                 const bool next = more;
-                acquire(&sm.k_empty[st], n);
-                if (!ok) break;
-                load.put_scales(now, sm.meta[n % kMetaStages]);
-                load.convert(kv, k_tile + st * Shape::kOperand, false);
-                fence_proxy_async_smem();
-                mbar_arrive(&sm.k_full[st]);
+                uint4 v[Loader::EACH];  // of keys, then of values: both at once do not fit the registers
+                load.fetch(a.cache.k.p, now.k, v);
                 if (next) {
-                    load.put_there(place, sm.meta[(n + 1) % kMetaStages]);
                     rows = load.find(place);
-                    load.fetch(a.cache.k.p, rows.k, kv);
+                    load.put_there(place, sm.meta[(n + 1) % kMetaStages]);
                     more = step();
                     if (more) place = load.look_up(it, key0());
                 }
+                acquire(&sm.k_empty[st], n);
+                if (!ok) break;
+                load.put_scales(now, sm.meta[n % kMetaStages]);
+                load.convert(v, k_tile + st * Shape::kOperand, false);
+                load.fetch(a.cache.v.p, now.v, v);
+                fence_proxy_async_smem();
+                mbar_arrive(&sm.k_full[st]);
                 acquire(&sm.v_empty[st], n);
                 if (!ok) break;
-                if (load.convert(vv, v_tile + st * Shape::kOperand, !now.whole)) sm.odd = 1;
+                if (load.convert(v, v_tile + st * Shape::kOperand, !now.whole)) sm.odd = 1;
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.v_full[st]);
                 if (!next) break;
-                load.fetch(a.cache.v.p, rows.v, vv);
             }
         }
         cp_async_wait_everything();
@@ -689,10 +687,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                         for (int c = 0; c < kTilesKeys; c += 4) {
                             const float4 kc = *reinterpret_cast<const float4*>(meta.kc + c);
                             const float4 lv = *reinterpret_cast<const float4*>(meta.lv + c);
-                            x[c] = fmaf(x[c], kc.x * my_factor, lv.x);
-                            x[c + 1] = fmaf(x[c + 1], kc.y * my_factor, lv.y);
-                            x[c + 2] = fmaf(x[c + 2], kc.z * my_factor, lv.z);
-                            x[c + 3] = fmaf(x[c + 3], kc.w * my_factor, lv.w);
+                            float2 k0 = make_float2(kc.x, kc.y), k1 = make_float2(kc.z, kc.w);
+                            if constexpr (!std::is_same_v<T, __half>) {
+                                k0 = mul2(k0, make_float2(my_factor, my_factor));
+                                k1 = mul2(k1, make_float2(my_factor, my_factor));
+                            }
+                            const float2 x0 = fma2(make_float2(x[c], x[c + 1]), k0, make_float2(lv.x, lv.y));
+                            const float2 x1 = fma2(make_float2(x[c + 2], x[c + 3]), k1, make_float2(lv.z, lv.w));
+                            x[c] = x0.x;
+                            x[c + 1] = x0.y;
+                            x[c + 2] = x1.x;
+                            x[c + 3] = x1.y;
                         }
                     }
                     if (!whole) {
