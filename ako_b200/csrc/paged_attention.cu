@@ -68,7 +68,9 @@ extern "C" int ako_b200_paged_attention(const void* q, int64_t q_stride_b, int64
     if (rc) return rc;
     if (window < 0 || sinks < 0)
         return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: window and sinks must be >= 0", op);
-    if (!std::isfinite(scale)) return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: scale must be finite", op);
+    a.scale = static_cast<float>(scale * 1.4426950408889634);
+    if (!std::isfinite(a.scale))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: scale must be finite, in fp32 too", op);
     if ((rc = refuse_if_wait_expired(op))) return rc;
     if (tokens == 0 || a.seqs.batch == 0) return AKO_B200_OK;
     if (q == nullptr || out == nullptr)
@@ -93,11 +95,10 @@ extern "C" int ako_b200_paged_attention(const void* q, int64_t q_stride_b, int64
     // A window that reaches behind every position is none.
     a.window = static_cast<int>(window >= a.seqs.max_kv ? 0 : window);
     a.sinks = static_cast<int>(a.window == 0 ? 0 : sinks < a.seqs.max_kv ? sinks : a.seqs.max_kv);
-    a.scale = static_cast<float>(scale * 1.4426950408889634);
     a.joins = static_cast<int4*>(workspace);
     a.partial = reinterpret_cast<float*>(a.joins + p.ctas);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return p.kernel == 0 ? launch_rows(a, p, st) : launch_tiles(a, p, scale, st);
+    return p.kernel == 0 ? launch_rows(a, p, st) : launch_tiles(a, p, st);
 }
 
 extern "C" int ako_b200_paged_attention_plan(const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,

@@ -36,8 +36,8 @@ inline int64_t attention_workspace(int ctas, int rows, bool wide) {
 void plan_rows(AttnPlan& p);
 int launch_rows(const AttnArgs& a, const AttnPlan& p, cudaStream_t st);
 
-// Kernel 1, on the tensor cores; `scale` is the call's, with its sign.
+// Kernel 1, on the tensor cores.
 void plan_tiles(AttnPlan& p);
-int launch_tiles(const AttnArgs& a, const AttnPlan& p, double scale, cudaStream_t st);
+int launch_tiles(const AttnArgs& a, const AttnPlan& p, cudaStream_t st);
 
 }  // namespace ako_b200

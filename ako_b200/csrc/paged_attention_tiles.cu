@@ -79,16 +79,16 @@ void plan_tiles(AttnPlan& p) {
     p.workspace = attention_workspace(p.ctas, kTilesRows, p.wide);
 }
 
-int launch_tiles(const AttnArgs& a, const AttnPlan& p, double scale, cudaStream_t st) {
+int launch_tiles(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
     TilesArgs t{};
     t.a = a;
     t.status = device_status_word();
     t.wait_polls = wait_polls();
-    t.q_factor = scale < 0 ? -1.0f : scale == 0 ? 0.0f : 1.0f;
+    t.q_factor = a.scale < 0 ? -1.0f : a.scale == 0 ? 0.0f : 1.0f;
     if (t.status == nullptr) return AKO_B200_ERR_CUDA;
     // The softmax follows the largest score, so the scale's sign goes into q;
     // a scale of zero is a q of zero.
-    t.a.scale = scale == 0 ? 1.0f : std::fabs(a.scale);
+    t.a.scale = a.scale == 0 ? 1.0f : std::fabs(a.scale);
     // Boxes start on multiples of eight rows, the swizzle's period, and 64 rows are made of whole ones.
     const int page = a.cache.page_size;
     if (!p.quant && page % 8 == 0 && (page % 64 == 0 || 64 % page == 0)) {

@@ -49,10 +49,14 @@ def _strides(t: torch.Tensor) -> tuple[int, ...]:
 
 def _vectors(t: torch.Tensor) -> torch.Tensor:
     """``t`` with a contiguous last axis and all else on 16-byte boundaries, copied only if it is not so."""
-    each = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % each == 0 for s in _strides(t)[:-1]):
-        return t
-    return t.contiguous()
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():  # rows of whole vectors, one behind the other
+            return t
+        each = 16 // t.element_size()
+        if t.stride(-1) == 1 and all(s % each == 0 for s in _strides(t)[:-1]):
+            return t
+    out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return out.copy_(t)
 
 
 class PagedKV:
@@ -100,7 +104,6 @@ class PagedKV:
             k.data_ptr(), v.data_ptr(), scales[0][0], scales[1][0], *_strides(k)[:3], *_strides(v)[:3],
             *scales[0][1], *scales[1][1], pages, heads, page_size, dim, code)
         self._ref = ctypes.byref(self._c)
-        self._key = (self.dtype, heads, page_size, dim, self.device)
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, *, dtype: torch.dtype,
@@ -158,7 +161,6 @@ class PagedBatch:
             page_table.data_ptr(), kv_lens.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
             page_table.stride(0) if batch > 1 else pages, batch, pages, self._most)
         self._ref = ctypes.byref(self._c)
-        self._key = (batch, pages, cu_seqlens is None, self._most)
 
 
 def _check(cache: PagedKV, batch: PagedBatch, fn: str) -> None:
@@ -258,21 +260,24 @@ def kv_cache_read_cuda_sm100(
     return k, v
 
 
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(cache_key: tuple, batch_key: tuple, tokens: int, q_len: int, q_heads: int, code: int) -> int:
-    """Workspace that a call of these sizes needs; sizes alone decide it."""
-    dtype, kv_heads, page_size, dim, device = cache_key
-    batch, pages, uniform, most = batch_key
+#: Rows from which on the kernel, and with it the workspace, is always the same.
+_MANY_ROWS = 1024
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(dtype: torch.dtype, dim: int, device: torch.device, code: int, rows: int) -> int:
+    """Workspace of a call whose longest sequence has ``rows`` rows (new tokens times q heads per kv head): the rows,
+    the types and the head's width alone decide it, so one token of a cache with one head stands for them."""
     p = 256  # an aligned address, never read
     quantised = dtype == E4M3
-    kv = _native.PagedKVStruct(p, p, p if quantised else None, p if quantised else None, *([0] * 12), 1, kv_heads,
-                               page_size, dim, _E4M3_CODE if quantised else _DTYPE_CODE[dtype])
-    seqs = _native.PagedBatchStruct(p, p, None if uniform else p, pages, batch, pages, most)
-    kernel, rows, ctas, size = ctypes.c_int(), ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
+    kv = _native.PagedKVStruct(p, p, p if quantised else None, p if quantised else None, *([0] * 12), 1, 1, 16, dim,
+                               _E4M3_CODE if quantised else _DTYPE_CODE[dtype])
+    seqs = _native.PagedBatchStruct(p, p, None, 1, 1, 1, 1)
+    kernel, tile, ctas, size = ctypes.c_int(), ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
     with _DeviceGuard(device):
         status = _native.active().ako_b200_paged_attention_plan(
-            ctypes.byref(kv), ctypes.byref(seqs), tokens, q_len, q_heads, code, ctypes.byref(kernel),
-            ctypes.byref(rows), ctypes.byref(ctas), ctypes.byref(size))
+            ctypes.byref(kv), ctypes.byref(seqs), 1, 1, rows, code, ctypes.byref(kernel), ctypes.byref(tile),
+            ctypes.byref(ctas), ctypes.byref(size))
     _native.raise_for_status(status, "paged_attention_cuda_sm100")
     return size.value
 
@@ -319,7 +324,9 @@ def paged_attention_cuda_sm100(
         raise ValueError(f"{fn}: out must match q in shape, dtype and device and have a contiguous last axis")
     os = out.stride()
     os = (os[0], os[1], os[2]) if batch.cu_seqlens is None else (0, os[0], os[1])
-    size = _workspace_bytes(cache._key, batch._key, tokens, q_len, heads, code)
+    most = q_len if batch.cu_seqlens is None else min(batch._most, tokens)
+    rows = min(max(most, 1) * (heads // cache.kv_heads), _MANY_ROWS)
+    size = _workspace_bytes(cache.dtype, cache.head_dim, cache.device, code, rows)
     work = torch.empty(size, dtype=torch.uint8, device=q.device)
     with _DeviceGuard(q.device):
         status = _native.active().ako_b200_paged_attention(

@@ -108,7 +108,7 @@ def test_read_refusals(lib) -> None:
 def test_attention_refusals(lib) -> None:
     for kw, words in (({"heads": 3}, b"multiple of kv_heads"), ({"heads": 0}, b"multiple of kv_heads"),
                       ({"window": -1}, b"window"), ({"sinks": -1}, b"sinks"), ({"scale": float("nan")}, b"scale"),
-                      ({"scale": float("inf")}, b"scale"), ({"q": None}, b"null"), ({"out": None}, b"null"),
+                      ({"scale": float("inf")}, b"scale"), ({"scale": 1e39}, b"scale"), ({"q": None}, b"null"), ({"out": None}, b"null"),
                       ({"q": P + 8}, b"16 bytes"), ({"stride": 252}, b"16 bytes"), ({"work": None}, b"workspace"),
                       ({"work": P + 8}, b"workspace"), ({"size": 100}, b"workspace")):
         assert attention(lib, cache(), seqs(), **kw) == 1
@@ -131,6 +131,8 @@ def test_plan_goes_by_the_rows_of_a_sequence(lib) -> None:
     assert _plan(lib, cache(), seqs(), 3, 1, 16)[:2] == (0, 8)
     assert _plan(lib, cache(), seqs(), 3, 1, 20)[:2] == (0, 16)
     assert _plan(lib, cache(), seqs(), 6, 2, 32)[:2] == (0, 32)
+    assert _plan(lib, cache(), seqs(), 6, 2, 34)[:2] == (1, 256)
+    assert _plan(lib, cache(), seqs(cu_seqlens=P, max_q_len=5), 30, 0, 14)[:2] == (1, 256)
     packed = seqs(cu_seqlens=P, max_q_len=4)
     assert _plan(lib, cache(), packed, 30, 0, 4)[:2] == (0, 8)
     kernel, rows, ctas, size = _plan(lib, cache(), seqs(), 3, 1, 16)

@@ -197,16 +197,47 @@ def test_attention_with_pages_given_away(cuda_device) -> None:
     check_attention(p, want, window=50, sinks=3)
 
 
-def test_attention_rows_without_keys_are_zero(cuda_device) -> None:
+@pytest.mark.parametrize("more", [0, 150], ids=["few", "many"])
+@pytest.mark.parametrize("quantised", [False, True], ids=["same", "e4m3"])
+def test_attention_rows_without_keys_are_zero(cuda_device, quantised, more) -> None:
     """More new tokens than cached ones, no cached ones, no new ones, and only pages that are not there."""
-    p = Problem(BF16, False, 4, 2, 64, 16, [(5, 5), (3, 3), (0, 9), (2, 10)], True, 15, cuda_device)
-    p.kv_lens[0] = 2  # three rows before the first position
+    n = 5 + more
+    p = Problem(BF16, quantised, 4, 2, 64, 16, [(n, n), (3, 3), (0, 9), (2, 10)], True, 15, cuda_device)
+    p.kv_lens[0] = 2  # all rows but two before the first position
     p.kv_lens[1] = 0
     p.table[3, 0] = -1
     out = _run(p).cpu()
-    assert bool((out[:3] == 0).all()) and bool((out[5:8] == 0).all()) and bool((out[8:] == 0).all())
-    want, bound = attend(p.q[3:5], p.k[0][:2], p.v[0][:2], p.v_scale[0][:2], sees(2, 2, 0, 0), 64**-0.5, BF16, False)
-    assert bool(((out[3:5].double() - want).abs() <= bound).all())
+    assert bool((out[: n - 2] == 0).all()) and bool((out[n:] == 0).all())
+    want, bound = attend(p.q[n - 2:n], p.k[0][:2], p.v[0][:2], p.v_scale[0][:2], sees(2, 2, 0, 0), 64**-0.5, BF16, quantised)
+    assert bool(((out[n - 2:n].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("new", [2, 100], ids=["few", "many"])
+def test_attention_clamps_what_it_is_told(cuda_device, new) -> None:
+    """Lengths past the table, negative ones and offsets past the tokens: what there is is attended, nothing else is
+    touched."""
+    p = Problem(BF16, False, 4, 2, 64, 16, [(new, 160), (new, 160), (new, 160), (new, 160)], True, 27, cuda_device)
+    want = _run(p)
+    p.kv_lens[0] = 2_000_000_000  # the table holds 160 positions
+    p.kv_lens[1] = -5
+    p.cu[4] = 1_000_000
+    out = torch.full((4 * new + 3, 4, 64), 9.0, dtype=BF16, device=cuda_device)
+    q = torch.cat([p.q.to(cuda_device), torch.zeros(3, 4, 64, dtype=BF16, device=cuda_device)])
+    p.cu[3] = 2 * new  # the third sequence has no new tokens, the fourth all the others
+    paged_attention_cuda_sm100(q, p.kv(), p.batch(), out=out)
+    assert torch.equal(out[:new], want[:new])
+    assert bool((out[new:2 * new] == 0).all())
+    assert torch.isfinite(out).all() and not bool((out[2 * new:] == 9).all(-1).any())
+    p.cu[:] = torch.tensor([4 * new, 3, -9, 2 * new, 2 * new])  # in no order
+    out.fill_(9.0)
+    paged_attention_cuda_sm100(q, p.kv(), p.batch(), out=out)
+    assert bool((out[2 * new:] == 9).all())
+
+
+def test_max_q_len_chooses_a_kernel_and_bounds_nothing(cuda_device) -> None:
+    p = Problem(BF16, False, 8, 2, 64, 16, [(70, 300), (1, 40), (9, 9)], True, 28, cuda_device)
+    check_attention(p, _run(p, max_q_len=1))
+    check_attention(p, _run(p, max_q_len=1000))
 
 
 @pytest.mark.parametrize("quantised", [False, True], ids=["same", "e4m3"])
@@ -238,18 +269,21 @@ def test_attention_large_scores_and_scales(cuda_device) -> None:
     """Scores of hundreds (weights of all but one key underflow), a negative scale, and keys' and values' scales far
     apart."""
     p = Problem(F16, False, 4, 2, 64, 16, [(3, 150), (1, 400)], True, 17, cuda_device, spread=20.0)
-    check_attention(p, _run(p, scale=1.0), scale=1.0)
-    check_attention(p, _run(p, scale=-0.25), scale=-0.25)
-    check_attention(p, _run(p, scale=0.0), scale=0.0)
-    p = Problem(BF16, True, 4, 2, 64, 16, [(3, 150), (1, 400)], True, 18, cuda_device)
-    for b, (_, kv) in enumerate(p.lengths):
-        for j in range(kv):
-            f = 2.0 ** ((j * 7) % 40 - 20)
-            at = int(p.table[b, j // 16]), slice(None), j % 16
-            p.caches["v_scale"][at] *= f
-            p.v[b][j] *= f
-            p.v_scale[b][j] *= f
-    check_attention(p, _run(p))
+    for scale in (1.0, -0.25, 0.0, 1e-60):
+        check_attention(p, _run(p, scale=scale), scale=scale)
+    p = Problem(F16, False, 4, 2, 64, 16, [(60, 150), (33, 400)], True, 17, cuda_device, spread=20.0)
+    for scale in (1.0, -0.25, 0.0, 1e-60):
+        check_attention(p, _run(p, scale=scale), scale=scale)
+    for lengths in ([(3, 150), (1, 400)], [(60, 150), (33, 400)]):
+        p = Problem(BF16, True, 4, 2, 64, 16, lengths, True, 18, cuda_device)
+        for b, (_, kv) in enumerate(p.lengths):
+            for j in range(kv):
+                f = 2.0 ** ((j * 7) % 40 - 20)
+                at = int(p.table[b, j // 16]), slice(None), j % 16
+                p.caches["v_scale"][at] *= f
+                p.v[b][j] *= f
+                p.v_scale[b][j] *= f
+        check_attention(p, _run(p))
 
 
 def test_attention_of_strided_queries_into_strided_outputs(cuda_device) -> None:
@@ -267,13 +301,14 @@ def test_attention_of_strided_queries_into_strided_outputs(cuda_device) -> None:
     assert torch.equal(paged_attention_cuda_sm100(odd[..., :64], p.kv(), p.batch()), want)
 
 
-def test_rows_behind_the_last_sequence_are_left(cuda_device) -> None:
-    p = Problem(BF16, False, 4, 2, 64, 16, [(3, 50), (2, 60)], True, 20, cuda_device)
+@pytest.mark.parametrize("new", [3, 90], ids=["few", "many"])
+def test_rows_behind_the_last_sequence_are_left(cuda_device, new) -> None:
+    p = Problem(BF16, False, 4, 2, 64, 16, [(new, 100), (2, 60)], True, 20, cuda_device)
     want = _run(p)
     q = torch.cat([p.q.to(cuda_device), torch.full((4, 4, 64), math.nan, dtype=BF16, device=cuda_device)])
     out = torch.full_like(q, 5.0)
     paged_attention_cuda_sm100(q, p.kv(), p.batch(), out=out)
-    assert torch.equal(out[:5], want) and bool((out[5:] == 5).all())
+    assert torch.equal(out[: new + 2], want) and bool((out[new + 2:] == 5).all())
 
 
 def test_many_sequences(cuda_device) -> None:
@@ -311,7 +346,8 @@ def test_nothing_to_do(cuda_device) -> None:
     assert bool((kv_cache_read_cuda_sm100(cache, bare, 0, 2)[0] == 0).all())
 
 
-def test_offsets_beyond_32_bits(cuda_device) -> None:
+@pytest.mark.parametrize("new", [1, 40], ids=["few", "many"])
+def test_offsets_beyond_32_bits(cuda_device, new) -> None:
     """A cache of 2^32 + elements: its last pages lie behind 2^31 elements and 2^32 bytes."""
     pages, heads, page, dim = 33_000, 8, 64, 128  # 2.16e9 elements, 4.3 GB each in bf16
     k = torch.empty(pages, heads, page, dim, dtype=BF16, device=cuda_device)
@@ -324,10 +360,10 @@ def test_offsets_beyond_32_bits(cuda_device) -> None:
     got_k, got_v = kv_cache_read_cuda_sm100(cache, batch, 0, 150)
     assert torch.equal(got_k[0].transpose(0, 1).cpu(), new_k[0]) and torch.equal(got_v[0].transpose(0, 1).cpu(), new_v[0])
     assert torch.equal(k[pages - 2, :, 21].cpu(), new_k[0, 149])
-    q = torch.randn(1, 1, heads, dim, generator=g).to(BF16)
+    q = torch.randn(1, new, heads, dim, generator=g).to(BF16)
     out = paged_attention_cuda_sm100(q.to(cuda_device), cache, batch)
     want, bound = attend(q[0], new_k[0].double(), new_v[0].double(), torch.ones(150, heads, dtype=torch.float64),
-                         sees(1, 150, 0, 0), dim**-0.5, BF16, False)
+                         sees(new, 150, 0, 0), dim**-0.5, BF16, False)
     assert bool(((out[0].cpu().double() - want).abs() <= bound).all())
 
 
@@ -405,6 +441,27 @@ def test_graph_replay_on_new_contents_and_streams(cuda_device) -> None:
             k, _ = kv_cache_read_cuda_sm100(caches[i], batches[i], 0, 96)
             for b, n in enumerate(batches[i].kv_lens.tolist()):
                 assert torch.equal(k[b, :, n - 1], ks[i][b, 0])
+
+
+def test_graph_of_chunks_replayed_on_new_lengths(cuda_device) -> None:
+    """Chunks on the tensor cores, captured without a call before, replayed with other lengths and another split of
+    the tokens among the sequences."""
+    p = Problem(BF16, False, 8, 2, 128, 32, [(50, 300), (40, 90), (6, 500)], True, 29, cuda_device)
+    q, cache, batch = p.q.to(cuda_device), p.kv(), p.batch()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = paged_attention_cuda_sm100(q, cache, batch)
+    graph.replay()
+    check_attention(p, out)
+    other = [(10, 200), (80, 80), (6, 450)]
+    batch.kv_lens.copy_(torch.tensor([kv for _, kv in other]))
+    batch.cu_seqlens.copy_(torch.tensor([0, 10, 90, 96]))
+    graph.replay()
+    p.cu, p.lengths = torch.tensor([0, 10, 90, 96]), other
+    for b, (_, kv) in enumerate(other):
+        p.k[b], p.v[b], p.v_scale[b] = p.k[b][:kv], p.v[b][:kv], p.v_scale[b][:kv]
+    check_attention(p, out)
 
 
 def test_same_bits_twice_and_on_another_stream(cuda_device) -> None:
