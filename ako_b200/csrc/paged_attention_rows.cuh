@@ -84,10 +84,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// Two e4m3 values, the low 16 bits of `pair`, as two fp16 (exact).
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t pair) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(pair));
+// Four e4m3 values as two pairs of fp16 (exact).
+__device__ __forceinline__ uint2 e4m3x4_to_half2x2(uint32_t four) {
+    uint2 r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(r.x), "=r"(r.y)
+        : "r"(four));
     return r;
 }
 
@@ -360,8 +363,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                     const uint32_t u[4] = {lo.x, lo.y, lo.z, lo.w}, w[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t kf[4] = {e4m3x2_to_half2(u[i]), e4m3x2_to_half2(w[i]),
-                                                e4m3x2_to_half2(u[i] >> 16), e4m3x2_to_half2(w[i] >> 16)};
+                        const uint2 f = e4m3x4_to_half2x2(u[i]), f8 = e4m3x4_to_half2x2(w[i]);
+                        const uint32_t kf[4] = {f.x, f8.x, f.y, f8.y};
                         scores(j * 4 + i, kf);
                     }
                 }
@@ -539,8 +542,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                             uint32_t vf[4];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                vf[2 * e] = e4m3x2_to_half2(__byte_perm(vr[i][2 * k + e], 0, 0x4420));
-                                vf[2 * e + 1] = e4m3x2_to_half2(__byte_perm(vr[i][2 * k + e], 0, 0x4431));
+                                const uint2 f = e4m3x4_to_half2x2(__byte_perm(vr[i][2 * k + e], 0, 0x3120));
+                                vf[2 * e] = f.x;
+                                vf[2 * e + 1] = f.y;
                             }
                             values(2 * (first + i) + k, vf);
                         }

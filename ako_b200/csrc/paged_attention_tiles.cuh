@@ -287,8 +287,8 @@ struct TileLoader {
             const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                uint4 w = make_uint4(e4m3x2_to_half2(u[2 * half]), e4m3x2_to_half2(u[2 * half] >> 16),
-                                     e4m3x2_to_half2(u[2 * half + 1]), e4m3x2_to_half2(u[2 * half + 1] >> 16));
+                const uint2 lo = e4m3x4_to_half2x2(u[2 * half]), hi = e4m3x4_to_half2x2(u[2 * half + 1]);
+                uint4 w = make_uint4(lo.x, lo.y, hi.x, hi.y);
                 if (clean && scrub<__half>(w)) any = true;
                 *reinterpret_cast<uint4*>(tile + place(rows0 + row0 + i * ROWS, chunk * 2 + half)) = w;
             }
