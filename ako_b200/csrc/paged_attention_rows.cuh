@@ -11,7 +11,10 @@
 // an N of 8 and not an M of 16. S^T's accumulators become P^T's operand by one
 // 8x8 transpose in registers (movmatrix).
 //
-// Bound: HBM, by the keys and values read once.
+// Bound: HBM, by the keys and values read once. 32 contexts of 2048 tokens (32
+// heads of 128, 8 kv heads, bf16, 252 MB): 51 us, 4.9 TB/s with the launch's
+// begin and end; 16 e4m3 contexts of 2000 to 65536 tokens (849 MB): 156 us,
+// 5.4 TB/s, where conversions take 0.6 of the issue slots.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -24,7 +27,9 @@ constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kWarpKeys = 16;
 constexpr int kRowsKeys = kRowsWarps * kWarpKeys;  // keys of a tile
-constexpr int kRowsCost = 2;                       // tiles that an item's begin and end take as long as
+// Tiles that an item's begin and end take as long as. 64 sequences under a window of 1024: 15.4 us
+// with 2 or 3, 17.1 with 1, 19.7 with 0.
+constexpr int kRowsCost = 2;
 
 // 16-byte asynchronous copy; zeros instead when `real` is false.
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool real) {

@@ -202,11 +202,11 @@ int ako_b200_rmsnorm_plan(int64_t n_rows, int64_t hidden_dim, int dtype, int res
                           int* kernel, int* cluster, int* threads_per_row, int* vectors_per_thread);
 
 /*
- * Status of the persistent RMSNorm kernels (the staged and chunked kernels,
- * which wait on 1-D bulk copies). Every such wait is bounded (about a
- * second of polling). If one runs out, the kernel writes NaN into each
- * output row it could not produce (y, and residual_out for the fused form),
- * records the event in a status word in host-mapped memory, and exits. From
+ * Status of the kernels that wait: the persistent RMSNorm kernels (the staged
+ * and chunked kernels, which wait on 1-D bulk copies) and paged attention's
+ * kernel 1. Every such wait is bounded (about a second of polling). If one
+ * runs out, the kernel writes NaN into each output row it could not produce
+ * (y, and residual_out for the fused form; out), records the event in a status word in host-mapped memory, and exits. From
  * then on every entry point of this library refuses with
  * AKO_B200_ERR_WAIT_EXPIRED, before launching anything, so the expiry
  * surfaces at the next call without any synchronization on the hot path.
@@ -352,10 +352,15 @@ int ako_b200_paged_attention(const void* q, int64_t q_stride_b, int64_t q_stride
 /*
  * The kernel that a call with these arguments would run on the current device
  * (on 148 SMs where there is none), without launching anything and without
- * reading device memory: *kernel 0 is the one for few rows (warp-level matrix
- * instructions, *tile_rows rows of one sequence and kv head at a time), and
- * its grid of *ctas CTAs shares the sequences' key tiles out evenly, whatever
+ * reading device memory. A sequence's rows are its new tokens times the q
+ * heads that share a kv head. *kernel 0 is the one for sequences of at most 32
+ * rows (warp-level matrix instructions), 1 the one for more (tensor memory);
+ * *tile_rows rows of one sequence and kv head are taken at a time, and a grid
+ * of *ctas CTAs shares the key tiles of all sequences out evenly, whatever
  * their lengths. *workspace_bytes: what ako_b200_paged_attention needs.
+ *
+ * Kernel 1 waits on copies and products with a limit, as the persistent
+ * RMSNorm kernels do: see ako_b200_take_device_status.
  */
 int ako_b200_paged_attention_plan(const ako_b200_paged_kv* cache, const ako_b200_paged_batch* batch,
                                   int64_t tokens, int64_t q_len, int64_t q_heads, int dtype,
