@@ -17,6 +17,8 @@
 // 5.4 TB/s, where conversions take 0.6 of the issue slots.
 #pragma once
 
+#include <utility>
+
 #include <cuda_fp8.h>
 
 #include "paged_attention.cuh"
@@ -34,6 +36,13 @@ constexpr int kRowsCost = 2;
 // 16-byte asynchronous copy; zeros instead when `real` is false.
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(real ? 16 : 0)
+                 : "memory");
+}
+
+// The same without the choice, at constant offsets.
+template <int TO, int FROM>
+__device__ __forceinline__ void cp_async16_at(uint32_t smem, const void* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(smem), "l"(gmem), "n"(TO), "n"(FROM)
                  : "memory");
 }
 
@@ -120,7 +129,8 @@ struct RowsShape {
     static constexpr int kRows = NT * 8;
     static constexpr int kRowBytes = DPAD * (QUANT ? 1 : 2);
     static constexpr int kChunks = kRowBytes / 16;
-    static constexpr int kStageBytes = 2 * kWarpKeys * kRowBytes + (QUANT ? 2 * kWarpKeys * 4 : 0) + 16;
+    // keys, values, scales, and which keys are there; a multiple of 128, so that swizzles are exclusive ors
+    static constexpr int kStageBytes = 2 * kWarpKeys * kRowBytes + 2 * kWarpKeys * 4 + 128;
     // Warps on an SM count for more than stages: a warp's 16 keys are a chain of reads, products and
     // exponentials. Head 128: with 16 bits two CTAs of 3 stages 51 us a batch of 32 contexts of 2048
     // tokens, three of 2 stages 54, one of 4 stages 64; in e4m3 four CTAs of 3 stages 172 us where
@@ -144,6 +154,20 @@ __device__ __forceinline__ int swizzled(int row, int c) {
     if constexpr (!QUANT) return c ^ (row & 7);
     if constexpr (KEYS) return DPAD == 128 ? c ^ ((row & 1) << 2) : c;
     return DPAD == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3);
+}
+
+// Copies 16 rows that lie one behind the other, in the cache as in the stage:
+// every address is a lane's own and a constant. Row r of chunk c goes to chunk
+// swizzled(r, c), which differs from that of the lane's first row by an
+// exclusive or that the row's distance alone gives.
+template <bool QUANT, int DPAD, bool KEYS, int... I>
+__device__ __forceinline__ void copy_dense(uint32_t to, const uint8_t* from, int lane, std::integer_sequence<int, I...>) {
+    constexpr int ROWB = DPAD * (QUANT ? 1 : 2), CHUNKS = ROWB / 16, TAKEN = 32 / CHUNKS;
+    const int row = lane / CHUNKS, c = lane % CHUNKS;
+    const uint32_t first = to + row * ROWB + swizzled<QUANT, DPAD, KEYS>(row, c) * 16;
+    (cp_async16_at<I * TAKEN * ROWB, I * TAKEN * ROWB>(
+         first ^ (swizzled<QUANT, DPAD, KEYS>(I * TAKEN, 0) * 16), from),
+     ...);
 }
 
 template <typename T, bool QUANT, int DPAD, int NT>
@@ -180,6 +204,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
         // Lanes 0-15 look after the 16 keys' rows of K, lanes 16-31 of V.
         const PagedTensor& mine = lane < 16 ? a.cache.k : a.cache.v;
         const bool one_page = a.cache.page_size % kWarpKeys == 0;
+        const bool dense = one_page && dim == DPAD && a.cache.k.slot * 16 == ROWB && a.cache.v.slot * 16 == ROWB;
         int next_page = -1, next_slot = 0;
         auto look_up = [&](int t) {
             const int key = key_tile(it, t) * kRowsKeys + warp * kWarpKeys + (lane & 15);
@@ -194,7 +219,13 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                 const uint32_t to = ring_addr + stage * Shape::kStageBytes;
                 const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
                 constexpr int BYTES = QUANT ? 1 : 2, TAKEN = 32 / CHUNKS;  // rows that the warp takes at once
-                if (one_page && there == 0xffffu) {
+                if (dense && there == 0xffffu) {
+                    using Times = std::make_integer_sequence<int, kWarpKeys / TAKEN>;
+                    const int first = slot - (lane & 15);  // the first key's slot
+                    copy_dense<QUANT, DPAD, true>(to, a.cache.k.row(page, it.h, first) + lane * 16, lane, Times{});
+                    copy_dense<QUANT, DPAD, false>(to + kWarpKeys * ROWB, a.cache.v.row(page, it.h, first) + lane * 16, lane,
+                                                   Times{});
+                } else if (one_page && there == 0xffffu) {
                     // 16 rows of one page, a slot apart: no lane needs another's place.
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
