@@ -12,9 +12,11 @@
 // 8x8 transpose in registers (movmatrix).
 //
 // Bound: HBM, by the keys and values read once. 32 contexts of 2048 tokens (32
-// heads of 128, 8 kv heads, bf16, 252 MB): 51 us, 4.9 TB/s with the launch's
-// begin and end; 16 e4m3 contexts of 2000 to 65536 tokens (849 MB): 156 us,
-// 5.4 TB/s, where conversions take 0.6 of the issue slots.
+// heads of 128, 8 kv heads, bf16, 252 MB): 48 us, 5.2 TB/s with the launch's
+// begin and end; 16 e4m3 contexts of 2000 to 65536 tokens (849 MB): 149 us,
+// 5.7 TB/s. Instructions count for almost as much: addresses made of constants
+// took those two from 51 and 157 us (the latter, at the clock of a long run,
+// from 169).
 #pragma once
 
 #include <utility>
@@ -132,9 +134,9 @@ struct RowsShape {
     // keys, values, scales, and which keys are there; a multiple of 128, so that swizzles are exclusive ors
     static constexpr int kStageBytes = 2 * kWarpKeys * kRowBytes + 2 * kWarpKeys * 4 + 128;
     // Warps on an SM count for more than stages: a warp's 16 keys are a chain of reads, products and
-    // exponentials. Head 128: with 16 bits two CTAs of 3 stages 51 us a batch of 32 contexts of 2048
-    // tokens, three of 2 stages 54, one of 4 stages 64; in e4m3 four CTAs of 3 stages 172 us where
-    // three of 4 take 179, two of 6 216.
+    // exponentials. Head 128, before the copies of dense pages were shortened: with 16 bits two CTAs of
+    // 3 stages took 51 us for 32 contexts of 2048 tokens, three of 2 stages 54, one of 4 stages 64; in
+    // e4m3 four CTAs of 3 stages 172 us where three of 4 took 179, two of 6 216.
     static constexpr int kStages = 3;
     static constexpr int kRing = kRowsWarps * kStages * kStageBytes;
     static constexpr int kJoinStride = DPAD + 4;  // floats; keeps the four column groups on different banks
@@ -523,8 +525,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                 pf[nt][0] = transpose8x8(pack2<M>(x[nt][0], x[nt][1]));
                 pf[nt][1] = transpose8x8(pack2<M>(x[nt][2], x[nt][3]));
             }
-            auto values = [&](int mt, uint32_t(&vf)[4]) {
-                if (!whole) {
+            auto values = [&](auto check, int mt, uint32_t(&vf)[4]) {
+                if constexpr (check.value) {
                     // A weight of zero does not keep an infinity or NaN out of a product, so a
                     // value that is not finite is taken out of the operand and, for the rows that
                     // see it, counted by a product of its own.
@@ -564,31 +566,35 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma16816<M>(o[mt][nt], vf, pf[nt][0], pf[nt][1]);
             };
+            auto weigh = [&](auto check) {
 #pragma unroll
-            for (int first = 0; first < MATRICES; first += VAHEAD) {
-                if constexpr (NT != 1) read_values(first);
+                for (int first = 0; first < MATRICES; first += VAHEAD) {
+                    if constexpr (NT != 1) read_values(first);
 #pragma unroll
-                for (int i = 0; i < VAHEAD; ++i) {
-                    if constexpr (QUANT) {
-                        // A 16-bit element of V is the pair (2u, 2u + 1) of a tile's 16 head columns:
-                        // its transposed matrices give rows 2u and 2u + 1, which are taken as rows
-                        // u and u + 8 of the operand.
+                    for (int i = 0; i < VAHEAD; ++i) {
+                        if constexpr (QUANT) {
+                            // A 16-bit element of V is the pair (2u, 2u + 1) of a tile's 16 head columns:
+                            // its transposed matrices give rows 2u and 2u + 1, which are taken as rows
+                            // u and u + 8 of the operand.
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            uint32_t vf[4];
+                            for (int k = 0; k < 2; ++k) {
+                                uint32_t vf[4];
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint2 f = e4m3x4_to_half2x2(__byte_perm(vr[i][2 * k + e], 0, 0x3120));
-                                vf[2 * e] = f.x;
-                                vf[2 * e + 1] = f.y;
+                                for (int e = 0; e < 2; ++e) {
+                                    const uint2 f = e4m3x4_to_half2x2(__byte_perm(vr[i][2 * k + e], 0, 0x3120));
+                                    vf[2 * e] = f.x;
+                                    vf[2 * e + 1] = f.y;
+                                }
+                                values(check, 2 * (first + i) + k, vf);
                             }
-                            values(2 * (first + i) + k, vf);
+                        } else {
+                            values(check, first + i, vr[i]);
                         }
-                    } else {
-                        values(first + i, vr[i]);
                     }
                 }
-            }
+            };
+            if (whole) weigh(std::false_type{});
+            else weigh(std::true_type{});
             stage = stage == STAGES - 1 ? 0 : stage + 1;
             __syncwarp();  // the stage is read before the next copies into it
         }
