@@ -48,7 +48,7 @@ __device__ __forceinline__ void item_geometry(const AttnArgs& a, Item& it) {
     it.p_lo = before + static_cast<int>(a.by_group.div(it.row0));
     it.p_hi = before + static_cast<int>(a.by_group.div(it.row0 + it.rows - 1));
     const int end = max(it.p_hi + 1, 0);
-    it.win_lo = a.window > 0 ? max(it.p_lo - a.window + 1, 0) : 0;
+    it.win_lo = a.window > 0 ? max(max(it.p_lo, 0) - a.window + 1, 0) : 0;
     it.tile_lo = it.win_lo / BN;
     it.sink_tiles = min((min(a.sinks, end) + BN - 1) / BN, it.tile_lo);
     // an item without a key still has its rows to write: one tile, all masked

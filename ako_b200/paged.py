@@ -40,11 +40,18 @@ E4M3 = torch.float8_e4m3fn
 _E4M3_CODE = 3
 #: Widest head the operators take.
 MAX_HEAD_DIM = 128
+#: Above every position and number of tokens.
+_ENDLESS = (1 << 31) - 1
 
 
 def _strides(t: torch.Tensor) -> tuple[int, ...]:
     """Strides, with those of axes of one element (which never matter) as 0."""
     return tuple(s if n > 1 else 0 for s, n in zip(t.stride(), t.shape))
+
+
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether an output repeats its elements along an axis, so that which row is left there would be chance."""
+    return any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
 
 
 def _vectors(t: torch.Tensor) -> torch.Tensor:
@@ -68,7 +75,8 @@ class PagedKV:
     page_size, kv_heads, head_dim)`` is passed as its ``transpose(1, 2)``),
     all on 16-byte boundaries. ``k_scale`` and ``v_scale``: float32
     ``(num_pages, kv_heads, page_size)``, for a quantised cache only; a cached
-    value stands for ``element * scale``. ``head_dim`` is a multiple of 8 (16
+    value stands for ``element * scale``, scales being positive (attention takes
+    a value's below 2^-100 for that). ``head_dim`` is a multiple of 8 (16
     when quantised) up to 128; attention takes float16 and bfloat16 queries.
     """
 
@@ -156,7 +164,7 @@ class PagedBatch:
             raise ValueError(f"{fn}: max_q_len is a positive number given with cu_seqlens")
         self.page_table, self.kv_lens, self.cu_seqlens, self.max_q_len = page_table, kv_lens, cu_seqlens, max_q_len
         self.device, self.batch, self.max_pages = page_table.device, batch, pages
-        self._most = max_q_len if max_q_len is not None else (1 << 31) - 1
+        self._most = _ENDLESS if max_q_len is None else min(max_q_len, _ENDLESS)
         self._c = _native.PagedBatchStruct(
             page_table.data_ptr(), kv_lens.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
             page_table.stride(0) if batch > 1 else pages, batch, pages, self._most)
@@ -239,8 +247,8 @@ def kv_cache_read_cuda_sm100(
         raise ValueError(f"{fn}: a quantised cache is read as float32/float16/bfloat16, got dtype {dtype}")
     if not cache.quantised and dtype != cache.dtype:
         raise ValueError(f"{fn}: a {cache.dtype} cache is read as such, got dtype {dtype}")
-    if start < 0 or length < 0:
-        raise ValueError(f"{fn}: start and length must be >= 0, got {start} and {length}")
+    if not (0 <= start <= _ENDLESS and 0 <= length <= _ENDLESS):
+        raise ValueError(f"{fn}: start and length must be within 0 .. 2^31 - 1, got {start} and {length}")
     shape = (batch.batch, cache.kv_heads, length, cache.head_dim)
     if out is None:
         k = torch.empty(shape, dtype=dtype, device=cache.device)
@@ -248,9 +256,9 @@ def kv_cache_read_cuda_sm100(
     else:
         k, v = out
         for name, t in (("k", k), ("v", v)):
-            if t.shape != shape or t.dtype != dtype or t.device != cache.device or t.stride(-1) != 1:
+            if t.shape != shape or t.dtype != dtype or t.device != cache.device or t.stride(-1) != 1 or _overlaps(t):
                 raise ValueError(f"{fn}: the output for {name} must be {dtype} {shape} on {cache.device} with a "
-                                 f"contiguous last axis")
+                                 f"contiguous last axis and no axis expanded")
     with _DeviceGuard(cache.device):
         status = _native.active().ako_b200_kv_cache_read(
             cache._ref, batch._ref, start, length, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], code,
@@ -295,7 +303,8 @@ def paged_attention_cuda_sm100(
     kv_heads)``. ``scale`` defaults to ``head_dim ** -0.5``. With ``window`` w
     above 0 the token at position p sees the positions ``p - w + 1 .. p`` and,
     below them, the first ``sinks`` ones; pages that are neither may have been
-    given away, their table entries set to -1. A row that sees nothing is zero.
+    given away, their table entries set to -1. A row that sees nothing, or
+    nothing with a score above minus infinity, is zero.
 
     Values that are infinite or NaN reach the rows that see them and no others.
     ``out``: where to write, with a contiguous last axis and 16-byte aligned
@@ -314,14 +323,17 @@ def paged_attention_cuda_sm100(
         raise ValueError(f"{fn}: {heads} q heads are not a multiple of the cache's {cache.kv_heads} kv heads")
     if window < 0 or sinks < 0:
         raise ValueError(f"{fn}: window and sinks must be >= 0, got {window} and {sinks}")
+    window, sinks = min(window, _ENDLESS), min(sinks, _ENDLESS)  # one that reaches behind every position is none
     if scale is None:
         scale = cache.head_dim ** -0.5
     elif not math.isfinite(scale):
         raise ValueError(f"{fn}: scale must be finite, got {scale}")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1:
-        raise ValueError(f"{fn}: out must match q in shape, dtype and device and have a contiguous last axis")
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1
+          or _overlaps(out)):
+        raise ValueError(f"{fn}: out must match q in shape, dtype and device and have a contiguous last axis and no "
+                         f"axis expanded")
     os = out.stride()
     os = (os[0], os[1], os[2]) if batch.cu_seqlens is None else (0, os[0], os[1])
     most = q_len if batch.cu_seqlens is None else min(batch._most, tokens)

@@ -256,7 +256,7 @@ int ako_b200_swiglu_plan(int64_t n_rows, int64_t hidden_dim, int dtype, int alig
  * dtype is that of the activations, or AKO_B200_E4M3 with one fp32 scale per
  * token and head in k_scale and v_scale, (num_pages, kv_heads, page_size) with
  * free strides: a cached value stands for element * scale. Scales are
- * positive. k, v and all their strides are multiples of 16 bytes, head_dim a
+ * positive; attention takes a v_scale below 2^-100 for that. k, v and all their strides are multiples of 16 bytes, head_dim a
  * multiple of 8 (of 16 in an e4m3 cache) and at most 128.
  */
 typedef struct {
@@ -332,7 +332,8 @@ int ako_b200_kv_cache_read(const ako_b200_paged_kv* cache, const ako_b200_paged_
  * Attention of the new tokens over the cache, which holds them already:
  *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / (q_heads / kv_heads)]) v[j, ...]
  * over the keys j that token i, at position p, sees: j <= p, and with a
- * window w > 0 only j > p - w or j < sinks. A row that sees none is zero.
+ * window w > 0 only j > p - w or j < sinks. A row that sees none,
+ * or none with a score above minus infinity, is zero.
  * q and out are laid out as ako_b200_kv_cache_write's k and v, with q_heads
  * heads, in fp16 or bf16 (`dtype`). Scores, the softmax's maximum and sum and
  * the output's sum are fp32; the weights are rounded to the operands' 16-bit

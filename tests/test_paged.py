@@ -197,7 +197,10 @@ def test_wrapper_checks() -> None:
                 lambda: kv_cache_write_cuda_sm100(gpu(3, 2, 2, 64, dtype=torch.float16),
                                                   gpu(3, 2, 2, 64, dtype=torch.float16), kv, flat),
                 lambda: kv_cache_read_cuda_sm100(kv, flat, -1, 4), lambda: kv_cache_read_cuda_sm100(kv, flat, 0, -4),
+                lambda: kv_cache_read_cuda_sm100(kv, flat, 1 << 31, 4), lambda: kv_cache_read_cuda_sm100(kv, flat, 0, 1 << 64),
                 lambda: kv_cache_read_cuda_sm100(kv, flat, 0, 4, dtype=torch.float16),
+                lambda: kv_cache_read_cuda_sm100(kv, flat, 0, 4, out=(gpu(3, 2, 4, 64), gpu(3, 1, 4, 64).expand(3, 2, 4, 64))),
+                lambda: paged_attention_cuda_sm100(gpu(3, 2, 4, 64), kv, flat, out=gpu(1, 2, 4, 64).expand(3, 2, 4, 64)),
                 lambda: kv_cache_read_cuda_sm100(kv, flat, 0, 4, out=(gpu(3, 2, 4, 64), gpu(3, 2, 5, 64))),
                 lambda: paged_attention_cuda_sm100(gpu(3, 2, 3, 64), kv, flat),
                 lambda: paged_attention_cuda_sm100(gpu(3, 2, 0, 64), kv, flat),

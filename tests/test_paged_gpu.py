@@ -265,6 +265,33 @@ def test_attention_nonfinite_values_stay_with_the_rows_that_see_them(cuda_device
     check_attention(p, out)
 
 
+@pytest.mark.parametrize("new", [1, 40], ids=["few", "many"])
+def test_attention_rows_whose_scores_are_all_minus_infinity_are_zero(cuda_device, new) -> None:
+    """Of the first sequence's rows only the last key is infinite, of the second's all are."""
+    p = Problem(BF16, False, 4, 2, 64, 16, [(new, new), (new, new)], True, 17, cuda_device)
+    p.q[..., 0] = -1.0
+    for j in range(new):
+        for b in range(2):
+            p.caches["k"][int(p.table[b, j // 16]), :, j % 16] = 0.0
+            p.caches["k"][int(p.table[b, j // 16]), :, j % 16, 0] = math.inf if b == 1 or j == new - 1 else 0.0
+    # infinity times the other columns' zeros of k is none: a score is that of column 0
+    out = _run(p)
+    assert bool((p.rows(out, 1) == 0).all())
+    first = p.rows(out, 0)
+    assert bool(torch.isfinite(first).all())
+    if new > 1:  # the last row: the mean of the values before its own
+        want = p.v[0][: new - 1].mean(0).repeat_interleave(2, 0)
+        bound = (2 * HALF_STEP[BF16] + 2.0**-20) * p.v[0].abs().amax()
+        assert bool(((first[-1].double().cpu() - want).abs() <= bound).all())
+
+
+def test_windows_that_reach_behind_everything_are_none(cuda_device) -> None:
+    p = Problem(BF16, False, 4, 2, 64, 16, [(40, 90), (1, 70)], True, 18, cuda_device)
+    want = _run(p)
+    for window, sinks in ((1 << 31, 0), (1 << 70, 5), (90, 1 << 70), ((1 << 64) + 5, 0)):
+        assert torch.equal(_run(p, window=window, sinks=sinks), want)
+
+
 def test_attention_large_scores_and_scales(cuda_device) -> None:
     """Scores of hundreds (weights of all but one key underflow), a negative scale, and keys' and values' scales far
     apart."""
