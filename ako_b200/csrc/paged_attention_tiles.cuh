@@ -444,6 +444,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 }
                 before = whole;
             }
+            const bool more = advance();  // while the softmax is at the last tile
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (h >= halves || !ok) break;
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 if (elect_one()) mma_commit(&sm.o_full[h]);
             }
             if (elect_one()) mma_commit(&sm.v_empty[(n - 1) % STAGES]);
-            if (!advance()) break;
+            if (!more) break;
         } while (ok);
         // nothing of this CTA's is under way when it gives its tensor memory back
         if (elect_one()) mma_commit(&sm.drained);
@@ -683,7 +684,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tmem_fence_after();
-                if (t == t_end - 1) prepare_next();
                 if (rows) {
                     float x[kTilesKeys];
 #pragma unroll
@@ -781,6 +781,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 }
                 tmem_fence_before();
                 mbar_arrive(&sm.p_full[h][1]);
+                if (t == t_end - 1) prepare_next();  // while the last products run
             }
             if (!ok) {
                 following = share;
