@@ -598,15 +598,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             pos = real ? it.kv - it.n + static_cast<int>(a.by_group.div(it.row0 + r)) : it.p_hi;
             const int64_t mine = real ? row_offset(a, it, it.row0 + r, a.qb, a.qs, a.qh) : -1;
             if (!QUANT && args.q_factor == 1.0f) {  // as it is
-                int64_t o[TIMES];
-#pragma unroll
-                for (int i = 0; i < TIMES; ++i) o[i] = __shfl_sync(0xffffffffu, mine, i * TAKEN + lane / LANES);
-#pragma unroll
+#pragma unroll 4
                 for (int i = 0; i < TIMES; ++i) {
-                    const bool there = o[i] >= 0 && c * 8 < a.cache.head_dim;
+                    const int64_t o = __shfl_sync(0xffffffffu, mine, i * TAKEN + lane / LANES);
+                    const bool there = o >= 0 && c * 8 < a.cache.head_dim;
                     cp_async16_or_zero(smem_addr(my_q) + TileLoader<T, QUANT, DPAD>::place(
                                                              (warp & 3) * 32 + i * TAKEN + lane / LANES, c),
-                                       static_cast<const T*>(a.q) + (there ? o[i] + c * 8 : 0), there);
+                                       static_cast<const T*>(a.q) + (there ? o + c * 8 : 0), there);
                 }
                 mbar_arrive_copied(&sm.q_full[h]);
                 return;
@@ -809,34 +807,29 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
 #pragma unroll
                 for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
 #pragma unroll 1
-                for (int c0 = 0; c0 < DPAD; c0 += 64) {
-                    uint32_t o[64];
+                for (int c0 = 0; c0 < DPAD; c0 += 32) {
+                    uint32_t o[32];
                     tmem_load32(o_at + c0, o);
-                    tmem_load32(o_at + c0 + 32, o + 32);
                     tmem_wait_load();
                     if (begins && ends) {
 #pragma unroll
-                        for (int c = 0; c < 64; c += 32) {
+                        for (int i = 0; i < 4; ++i) {
+                            Packed<T, 8> y;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                Packed<T, 8> y;
-#pragma unroll
-                                for (int e = 0; e < 8; e += 2)
-                                    put2(y, e, __uint_as_float(o[c + i * 8 + e]) * inv,
-                                         __uint_as_float(o[c + i * 8 + e + 1]) * inv);
-                                put(i, *reinterpret_cast<uint4*>(&y));
-                            }
-                            __syncwarp();
-                            const int col = c0 + c + lane % 4 * 8;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (to[k] >= 0 && col < a.cache.head_dim)
-                                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to[k] + col) = get(k);
-                            __syncwarp();
+                            for (int e = 0; e < 8; e += 2)
+                                put2(y, e, __uint_as_float(o[i * 8 + e]) * inv, __uint_as_float(o[i * 8 + e + 1]) * inv);
+                            put(i, *reinterpret_cast<uint4*>(&y));
                         }
+                        __syncwarp();
+                        const int col = c0 + lane % 4 * 8;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (to[k] >= 0 && col < a.cache.head_dim)
+                                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to[k] + col) = get(k);
+                        __syncwarp();
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 64; c += 16) {
+                        for (int c = 0; c < 32; c += 16) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 put(i, make_uint4(o[c + i * 4], o[c + i * 4 + 1], o[c + i * 4 + 2], o[c + i * 4 + 3]));
