@@ -786,26 +786,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 more = next_item<kTilesRows, kTilesKeys>(a, following);
                 loaded = false;
             }
+            const int r = row0 + lane;
+            const bool real = r < it.rows, begins = t0 == 0, ends = t_end == it.tiles;
+            const int64_t mine = real ? row_offset(a, it, it.row0 + r, a.ob, a.os, a.oh) : -1;
+            int64_t to[4];  // rows that the lane writes eight columns of
+#pragma unroll
+            for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
             ok = ok && tile_wait(sm, &sm.o_full[h], no++ & 1, polls);
             ok = __all_sync(0xffffffffu, ok);
             tmem_fence_after();
-            const bool begins = t0 == 0, ends = t_end == it.tiles;
             if (rows) {
                 // 64 bytes of a row at a time go through shared memory, so that four lanes write them.
-                const int r = row0 + lane;
-                const bool real = r < it.rows;
                 Block* const block = reinterpret_cast<Block*>(a.partial) + 2 * blockIdx.x + (begins ? 1 : 0);
                 const float nan = __int_as_float(0x7fffffff);
                 const float inv = !ok ? nan : sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
-                const int64_t mine = real ? row_offset(a, it, it.row0 + r, a.ob, a.os, a.oh) : -1;
                 auto put = [&](int i, const uint4& v) { staging[lane * 4 + (i ^ (lane >> 1 & 3))] = v; };
                 auto get = [&](int k) {
                     const int to = k * 8 + lane / 4;
                     return staging[to * 4 + (lane % 4 ^ (to >> 1 & 3))];
                 };
-                int64_t to[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, mine, k * 8 + lane / 4);
 #pragma unroll 1
                 for (int c0 = 0; c0 < DPAD; c0 += 32) {
                     uint32_t o[32];
