@@ -25,6 +25,9 @@
 // numbers after the division by their sum, and fit the 16-bit types; O is then
 // rescaled rarely.
 //
+// Where items change, what the next one needs is found while the last products
+// run, and that code is kept short (8 prompts of 2048 tokens: 382 to 347 us).
+//
 // Bound: per tile and half, two products of 128 x 128 x head_dim take 8 *
 // head_dim cycles and the 16384 exponentials 1024 cycles of the SM's 16 a
 // cycle; for a head of 128 the two are equal, 2080 cycles a tile for both
@@ -32,8 +35,9 @@
 // scores' arrival to the last weights) and its products do not overlap, and
 // the halves' products wait for one another. 2048 new tokens on 16384 cached
 // ones, 32 heads of 128 and 8 kv heads: 498 us in bf16, 1.17 PFLOP/s; 851 us in
-// e4m3, where the conversion of a tile (four warps, through registers) and the
-// scales that the softmax reads take longer than the products.
+// e4m3, where the softmax reads three more numbers for each key from shared
+// memory and four warps convert every tile through registers. (Fetching values
+// while keys are converted made no difference: 865 us.)
 //
 // Every wait is bounded. If one runs out, all roles stop waiting, the rows not
 // yet written become NaN, and the status word is set.
@@ -47,9 +51,11 @@ namespace ako_b200 {
 constexpr int kTilesThreads = 512;
 constexpr int kTilesRows = 256;
 constexpr int kTilesKeys = 128;
-// Tiles that an item's begin and end take as long as: 13,000 cycles for its
-// queries, first scores, last products and output. Counting it when the work is
-// shared out took prompts of 8 x 2048 from 549 to 424 us.
+// Tiles that an item's begin and end take as long as: 9,000 cycles for its
+// queries, first scores, last products and output, most of them because this
+// code runs once an item and its instructions are no longer cached. Counting it
+// when the work is shared out took prompts of 8 x 2048 from 549 to 424 us; 2, 3
+// and 4 are within 1% of one another.
 constexpr int kTilesCost = 4;
 constexpr int kEarly = 96;  // keys whose weights are handed on before the tile's others
 // Tiles whose key data are kept: the loading warps find a tile's keys one tile
