@@ -52,8 +52,9 @@ constexpr int kTilesThreads = 512;
 constexpr int kTilesRows = 256;
 constexpr int kTilesKeys = 128;
 // Tiles that an item's begin and end take as long as: 9,000 cycles for its
-// queries, first scores, last products and output, most of them because this
-// code runs once an item and its instructions are no longer cached. Counting it
+// queries, first scores, last products and output, several times what their
+// instructions would take; likely they have left the instruction cache by the
+// time they run again, since making the code shorter helped. Counting it
 // when the work is shared out took prompts of 8 x 2048 from 549 to 424 us; 2, 3
 // and 4 are within 1% of one another.
 constexpr int kTilesCost = 4;
