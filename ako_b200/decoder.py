@@ -304,10 +304,20 @@ class GraphDecoder:
     cache under a position mask, or a paged cache up to the device's lengths, so
     the graph is valid for every step. Tokens are written to ``tokens[:, step]``
     on the device.
+
+    The steps' positions are the device's own, so what holds them is checked
+    here: a cache that ``steps`` tokens more do not fit into, or positions that
+    the model has no rotation for, raise ``ValueError``.
     """
 
     def __init__(self, model: "Decoder", cache: KVCache | PagedKVCache, first_token: torch.Tensor,
                  steps: int) -> None:
+        if steps < 1:
+            raise ValueError(f"GraphDecoder: steps must be >= 1, got {steps}")
+        if cache.length + steps > cache.max_len:
+            raise ValueError(f"KV cache holds {cache.max_len} positions, asked for {cache.length + steps}")
+        if cache.length + steps > model.cfg.max_seq_len:
+            raise ValueError(f"the model has {model.cfg.max_seq_len} positions, asked for {cache.length + steps}")
         self.model = model
         self.cache = cache
         dev = first_token.device
@@ -350,7 +360,8 @@ class GraphDecoder:
         side = torch.cuda.Stream(self.tok.device)
         side.wait_stream(torch.cuda.current_stream(self.tok.device))
         with torch.cuda.stream(side):
-            for _ in range(2):
+            for _ in range(2):  # both at the first step's position, which is there however few steps follow
+                self.reset()
                 self._step()
         torch.cuda.current_stream(self.tok.device).wait_stream(side)
         self.reset()
