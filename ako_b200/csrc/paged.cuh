@@ -11,6 +11,7 @@
 
 #include "common.cuh"
 #include "host.hpp"
+#include "lengths.hpp"
 
 namespace ako_b200 {
 
@@ -54,12 +55,13 @@ __device__ __forceinline__ void new_tokens(const PagedSeqs& s, int b, int& first
         first = b * s.q_len;
         n = s.q_len;
     } else {
-        first = min(max(s.cu[b], 0), s.tokens);
-        n = max(min(s.cu[b + 1], s.tokens) - first, 0);
+        const RowRange r = row_range(s.cu[b], s.cu[b + 1], s.tokens);
+        first = r.first;
+        n = r.n;
     }
 }
 
-__device__ __forceinline__ int cached_tokens(const PagedSeqs& s, int b) { return min(max(s.kv_lens[b], 0), s.max_kv); }
+__device__ __forceinline__ int cached_tokens(const PagedSeqs& s, int b) { return clamp_to(s.kv_lens[b], s.max_kv); }
 
 // Page number of position p (0 <= p < max_kv) of sequence b, or -1 if the
 // table's entry lies outside the cache.

@@ -1,0 +1,68 @@
+"""Lengths and offsets in device memory that hold anything: the kernels' own arithmetic on them (csrc/lengths.hpp), in
+constant expressions of the host's compiler, which accepts no overflow in one, and the kernels on a GPU."""
+
+from __future__ import annotations
+
+import itertools
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+from paged_oracle import Problem, check_attention
+
+from ako_b200 import kv_cache_write_cuda_sm100, paged_attention_cuda_sm100
+
+CSRC = Path(__file__).resolve().parent.parent / "ako_b200" / "csrc"
+MIN, MAX = -(1 << 31), (1 << 31) - 1
+ENDS = [MIN, MIN + 1, MIN + 300, -9, -1, 0, 1, 299, 300, 301, MAX - 1, MAX]
+
+
+def compiles(tmp_path, lines) -> None:
+    """The static assertions `lines` hold, and evaluating them overflows nowhere."""
+    src = tmp_path / "lengths.cpp"
+    literal = "constexpr int low = -2147483647 - 1;\n"
+    src.write_text('#include "lengths.hpp"\nusing namespace ako_b200;\n' + literal + "\n".join(lines) + "\n")
+    got = subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-fsyntax-only", f"-I{CSRC}", str(src)],
+                         capture_output=True, text=True)
+    assert got.returncode == 0, got.stderr[:2000]
+
+
+def text(x: int) -> str:
+    return "low" if x == MIN else str(x)
+
+
+def test_rows_of_any_two_offsets(tmp_path) -> None:
+    lines = []
+    for begin, end, tokens in itertools.product(ENDS, ENDS, (0, 1, 300, MAX)):
+        first, last = (min(max(x, 0), tokens) for x in (begin, end))
+        call = f"row_range({text(begin)}, {text(end)}, {text(tokens)})"
+        lines.append(f"static_assert({call}.first == {first} && {call}.n == {max(last - first, 0)}, \"\");")
+    compiles(tmp_path, lines)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [2, 300], ids=["few", "many"])
+def test_offsets_far_outside_the_tokens(cuda_device, new) -> None:
+    """An odd group of heads (5 to a kv head). Sequences whose offsets run backwards or far past either end own the
+    rows that lie between them and no others."""
+    p = Problem(torch.bfloat16, False, 10, 2, 64, 16, [(new, new + 30), (new, new + 30), (new, new + 30)], True, 31,
+                cuda_device)
+    want = paged_attention_cuda_sm100(p.q.to(cuda_device), p.kv(), p.batch())
+    check_attention(p, want)
+    owned = slice(2 * new, 3 * new)
+    for cu in ([new, MIN, 2 * new, 3 * new], [MAX, MIN, 2 * new, MAX], [MIN + new, MIN, 2 * new, MAX - 1]):
+        # the second sequence holds rows 0 .. 2 * new - 1 where its begin is below 0
+        p.cu = torch.tensor(cu, dtype=torch.int32)
+        out = torch.full((3 * new + 2, 10, 64), 9.0, dtype=torch.bfloat16, device=cuda_device)
+        q = torch.cat([p.q.to(cuda_device), torch.zeros(2, 10, 64, dtype=torch.bfloat16, device=cuda_device)])
+        if cu[3] > 3 * new:  # the last sequence then owns the two rows behind the others'
+            q, out = q[:3 * new], out[:3 * new]
+        paged_attention_cuda_sm100(q, p.kv(), p.batch(), out=out)
+        assert torch.equal(out[owned], want[owned])
+        assert bool(torch.isfinite(out).all()) and bool((out[3 * new:] == 9).all())
+        before = p.caches["k"].clone()
+        kv_cache_write_cuda_sm100(p.k_new.to(cuda_device), p.v_new.to(cuda_device), p.kv(), p.batch())
+        pages = [int(x) for x in p.table[0]]
+        assert torch.equal(p.caches["k"][pages].view(torch.int16), before[pages].view(torch.int16))  # the first has no rows
+        p.caches["k"].copy_(before)
