@@ -544,11 +544,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                     mbar_arrive(&full[st]);
                 }
             }
-            if (!ok) {  // copies by tensor map that no one waits for any more land before the CTA ends
-                const volatile int never = 0;
-                for (uint32_t u = n > STAGES ? n - STAGES : 0; u < n; ++u)
-                    wait_bounded(&full[u % STAGES], (u / STAGES) & 1, kDrainPolls, &never);
-            }
+            // The last stages' copies by tensor map land before the CTA ends, even where whoever was to use
+            // them has given up; cp.async's own wait below does not cover them.
+            const volatile int never = 0;
+            for (uint32_t u = n > STAGES ? n - STAGES : 0; u < n; ++u)
+                wait_bounded(&full[u % STAGES], (u / STAGES) & 1, kDrainPolls, &never);
         } else {
             typename Loader::Place place = load.look_up(it, key0());
             load.put_there(place, sm.meta[0]);
@@ -865,6 +865,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             if (!more) break;
             share = following;
         }
+        cp_async_wait_everything();  // rows of q that no product waited for
         asm volatile("bar.arrive 2, 416;" ::: "memory");
     }
 }
