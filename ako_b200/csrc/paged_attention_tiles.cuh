@@ -456,6 +456,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
             for (int h = 0; h < 2; ++h) {
                 if (h >= halves || !ok) break;
                 weigh(h, n - 1, t_end - 1 > t0);
+                if (!ok) break;  // the last product was not issued, so these rows are not to be had
                 if (elect_one()) mma_commit(&sm.o_full[h]);
             }
             if (elect_one()) mma_commit(&sm.v_empty[(n - 1) % STAGES]);

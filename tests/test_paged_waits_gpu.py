@@ -45,3 +45,18 @@ def test_calls_after_a_wait_that_ran_out_midway(cuda_device, kind) -> None:
             _limited(p, q, polls)
             assert torch.equal(paged_attention_cuda_sm100(q, p.kv(), p.batch()), want)
     assert _native.take_device_status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_rows_are_right_or_nan_when_a_wait_runs_out_midway(cuda_device, kind) -> None:
+    """Never sums that lack a tile: a row is what it always is, or NaN and the expiry is on record."""
+    with _native.measurement():
+        p = _problem(kind, cuda_device)
+        q = p.q.to(cuda_device)
+        want = paged_attention_cuda_sm100(q, p.kv(), p.batch())
+        for polls in POLLS:
+            out, expired = _limited(p, q, polls)
+            nan = out.isnan().all(-1)
+            assert bool(((out == want).all(-1) | nan).all()), f"{polls} polls"
+            assert expired or not bool(nan.any()), f"{polls} polls"
+    assert _native.take_device_status() == 0
