@@ -302,9 +302,11 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
     int first, n;
     new_tokens(a.seqs, static_cast<int>(b), first, n);
     const int at = static_cast<int>(t) - first;
-    const int pos = cached_tokens(a.seqs, static_cast<int>(b)) - n + at;
     int slot = 0, page = -1;
-    if (at_row < a.rows && at >= 0 && at < n && pos >= 0) page = page_of(a.seqs, a.cache, static_cast<int>(b), pos, slot);
+    if (at_row < a.rows && at >= 0 && at < n) {
+        const int pos = new_position(a.seqs.kv_lens[b], n, at, a.seqs.max_kv);
+        if (pos >= 0) page = page_of(a.seqs, a.cache, static_cast<int>(b), pos, slot);
+    }
     if constexpr (QUANT) {
         store_quantised(k, a.cache.k, a.cache.ks, page >= 0, page, h, slot, c, a.lanes_log2, active);
         store_quantised(v, a.cache.v, a.cache.vs, page >= 0, page, h, slot, c, a.lanes_log2, active);

@@ -18,4 +18,12 @@ constexpr RowRange row_range(int begin, int end, int tokens) {
     return {first, last > first ? last - first : 0};
 }
 
+// Position of new token `at` (0 <= at < n) of a sequence of kv_len tokens, the
+// n new ones included, or -1 where the `held` positions of its table have no
+// place for it. A length past the table moves no token onto an earlier one's place.
+constexpr int new_position(int kv_len, int n, int at, int held) {
+    const int p = (kv_len < 0 ? 0 : kv_len) - n + at;
+    return p >= 0 && p < held ? p : -1;
+}
+
 }  // namespace ako_b200

@@ -140,7 +140,9 @@ class PagedBatch:
     No call reads these tensors on the host. What they say is clamped to what
     there is: lengths to the table and to the tokens given; a page number
     outside the cache is a page that is not there, not written, read as zeros
-    and seen by no token. Rows behind ``cu_seqlens[-1]`` are left as they are.
+    and seen by no token. New tokens of a length past the table that the table
+    has no place for are not written. Rows behind ``cu_seqlens[-1]`` are left
+    as they are.
     """
 
     def __init__(self, page_table: torch.Tensor, kv_lens: torch.Tensor, *, cu_seqlens: torch.Tensor | None = None,

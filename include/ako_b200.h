@@ -302,7 +302,9 @@ typedef struct {
  * cu_seqlens, `tokens` rows (stride_b is not used); without, batch x q_len
  * rows, tokens = batch * q_len. Each row is kv_heads x head_dim, its last axis
  * contiguous. A token at a position before 0 (a sequence of fewer cached than
- * new tokens) is not stored. No two tokens of a call may share a slot.
+ * new tokens) is not stored, nor is one at a position past the table (a length
+ * that the table does not hold): no token takes an earlier one's place. No two
+ * tokens of a call may share a slot.
  *
  * An e4m3 cache takes round(x / s) to nearest even, where s, the scale stored
  * with it, is the least power of two with max|x| / s <= 448 over the token's

@@ -9,7 +9,7 @@ from pathlib import Path
 
 import pytest
 import torch
-from paged_oracle import Problem, check_attention
+from paged_oracle import Problem, check_attention, quantise
 
 from ako_b200 import kv_cache_write_cuda_sm100, paged_attention_cuda_sm100
 
@@ -39,6 +39,40 @@ def test_rows_of_any_two_offsets(tmp_path) -> None:
         call = f"row_range({text(begin)}, {text(end)}, {text(tokens)})"
         lines.append(f"static_assert({call}.first == {first} && {call}.n == {max(last - first, 0)}, \"\");")
     compiles(tmp_path, lines)
+
+
+def test_positions_of_any_length(tmp_path) -> None:
+    lines = []
+    for kv, n, held in itertools.product(ENDS, (1, 2, 300, MAX), (0, 1, 160, MAX - 4096)):
+        for at in {0, n // 2, n - 1}:
+            p = max(kv, 0) - n + at
+            lines.append(f"static_assert(new_position({text(kv)}, {n}, {at}, {held}) == {p if 0 <= p < held else -1}, \"\");")
+    compiles(tmp_path, lines)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantised", [False, True], ids=["same", "e4m3"])
+def test_tokens_past_the_table_take_no_earlier_place(cuda_device, quantised) -> None:
+    """Tables of four pages of 8: lengths that end at the table's end, past it by fewer tokens than are new, by as
+    many, and by far."""
+    for ragged in (False, True):
+        p = Problem(torch.bfloat16, quantised, 2, 2, 64, 8, [(4, 32)] * 5, ragged, 5, cuda_device)
+        lens = [32, 34, 36, 1000, MAX]
+        p.kv_lens = torch.tensor(lens, dtype=torch.int32)
+        before = p.caches["k"].cpu().clone()
+        kv_cache_write_cuda_sm100(p.k_new.to(cuda_device), p.v_new.to(cuda_device), p.kv(), p.batch())
+        after = p.caches["k"].cpu()
+        for b, n in enumerate(lens):
+            for j in range(32):
+                at = int(p.table[b, j // 8]), slice(None), j % 8
+                i = j - (n - 4)
+                if 0 <= i < 4:
+                    new = p.rows(p.k_new, b)[i]
+                    if quantised:
+                        new = quantise(new)[0]
+                    assert torch.equal(after[at].double(), new.double())
+                else:
+                    assert torch.equal(after.view(torch.uint8)[at], before.view(torch.uint8)[at])
 
 
 @pytest.mark.gpu
