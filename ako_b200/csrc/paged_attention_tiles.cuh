@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
     if (!find_share<kTilesRows, kTilesKeys, kTilesCost, kTilesThreads>(a, kTilesCost + 1, sm.scratch, share)) return;
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&sm.k_full[i], QUANT ? 128 : 64);
+            mbar_init(&sm.k_full[i], QUANT ? 128 : 64 + 2);  // 16 bits: two warps' copies, and the masks they note
             mbar_init(&sm.v_full[i], QUANT ? 128 : 64);
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
@@ -518,6 +518,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 if (!values) {
                     load.put_there(now0, sm.meta[n % kMetaStages]);
                     load.put_there(now1, sm.meta[n % kMetaStages], 32);
+                    // an arrival by cp.async hands on its copies, not what was stored before it
+                    if (lane == 0) mbar_arrive(&full[st]);
                 }
                 if (args.box != 0 && now0.whole && __all_sync(0xffffffffu, load.there(now0) && load.there(now1))) {
                     // Boxes of whole pages, or of 64 rows of one, a lane to each.
