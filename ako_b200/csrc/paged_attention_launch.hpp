@@ -1,6 +1,8 @@
 // Host side of the attention kernels: which one a call runs, and its launch.
 #pragma once
 
+#include <atomic>
+
 #include "paged_attention.cuh"
 
 namespace ako_b200 {
@@ -12,18 +14,22 @@ struct AttnPlan {
     int64_t workspace;  // bytes: an int4 per CTA, then two partial blocks per CTA
 };
 
-// Raises a kernel's limit of dynamic shared memory once per device.
+constexpr int kMostDevices = 64;  // that launches remember something of
+using PerDevice = std::atomic<bool>[kMostDevices];
+
+// Raises a kernel's limit of dynamic shared memory once per device. Any number of threads may call
+// it at once: the limit is then raised more than once, to the same value.
 template <typename K>
-int allow_smem(K kernel, int bytes, bool (&done)[64], const char* name) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (done[dev]) return AKO_B200_OK;
+int allow_smem(K kernel, int bytes, PerDevice& done, const char* name) {
+    int dev = -1;
+    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMostDevices;
+    if (known && done[dev].load(std::memory_order_relaxed)) return AKO_B200_OK;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_error(AKO_B200_ERR_CUDA, "%s: %d bytes of shared memory: %s", name, bytes, cudaGetErrorString(e));
     }
-    done[dev] = true;
+    if (known) done[dev].store(true, std::memory_order_relaxed);
     return AKO_B200_OK;
 }
 

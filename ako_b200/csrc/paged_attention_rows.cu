@@ -8,7 +8,7 @@ namespace {
 template <typename T, bool QUANT, int DPAD, int NT>
 int launch(const AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
     using Shape = RowsShape<T, QUANT, DPAD, NT>;
-    static bool done[64] = {};
+    static PerDevice done{};
     const char* name = "paged_attention";
     int rc = allow_smem(attn_rows_kernel<T, QUANT, DPAD, NT>, Shape::kSmem, done, name);
     if (rc) return rc;

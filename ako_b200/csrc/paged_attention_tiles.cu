@@ -41,8 +41,9 @@ int launch(const TilesArgs& t, const AttnPlan& p, cudaStream_t st) {
     using Shape = TilesShape<DPAD>;
     const char* name = "paged_attention";
     auto kernel = attn_tiles_kernel<T, QUANT, DPAD>;
-    static bool done[64] = {};
-    static int regs = 0;
+    static PerDevice done{};
+    static std::atomic<int> launch_regs{0};
+    int regs = launch_regs.load(std::memory_order_relaxed);
     if (regs == 0) {
         // The warps' registers are shares of what the block is launched with.
         cudaFuncAttributes f{};
@@ -52,6 +53,7 @@ int launch(const TilesArgs& t, const AttnPlan& p, cudaStream_t st) {
             return set_error(AKO_B200_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
         }
         regs = f.numRegs;
+        launch_regs.store(regs, std::memory_order_relaxed);
     }
     if (regs * kTilesThreads < 128 * (2 * kSoftmaxRegs + kLoadRegs + kIssueRegs))
         return set_error(AKO_B200_ERR_CUDA, "%s: built with %d registers a thread, too few to share out", name, regs);
