@@ -240,6 +240,13 @@ struct PartialBlock {
 // rescaled rarely.
 constexpr float kGrowth = 8.0f;
 
+// A key of an e4m3 cache whose values are all zero, of score s (in powers of
+// two), has a weight and no values: its scale is any number. Rows' maxima, which
+// are those of score + log2(scale), follow such a key as if its scale were 2^-64:
+// its weight is then at most 2^(64 + kGrowth) in the sum, which stays finite, and
+// keys with values keep their 16 bits unless they contribute 2^-64 of it.
+constexpr float kEmptyBelow = 64.0f;
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -172,6 +172,21 @@ __device__ __forceinline__ void copy_dense(uint32_t to, const uint8_t* from, int
      ...);
 }
 
+// An e4m3 cache's values that are all zero (of either sign): bit r for row r of the 32 / CHUNKS * N
+// rows whose 16-byte chunks a warp holds, lane L chunk L % CHUNKS of rows L / CHUNKS + i * (32 / CHUNKS).
+template <int CHUNKS, int N>
+__device__ __forceinline__ uint32_t empty_rows(const uint4 (&v)[N]) {
+    constexpr int TAKEN = 32 / CHUNKS;
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    uint32_t held = 1;  // of the lane's row, a chunk with something in it; lanes past the rows count as held
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t any = __ballot_sync(0xffffffffu, ((v[i].x | v[i].y | v[i].z | v[i].w) & 0x7f7f7f7fu) != 0);
+        if (lane / TAKEN == i) held = any >> (lane % TAKEN * CHUNKS) & ((1u << CHUNKS) - 1u);
+    }
+    return __ballot_sync(0xffffffffu, held == 0);
+}
+
 template <typename T, bool QUANT, int DPAD, int NT>
 __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::kCtas))
     attn_rows_kernel(const AttnArgs a) {
@@ -444,10 +459,12 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
             if constexpr (NT == 1) read_values(0);
 
             // Scores in units of log2(e). A quantised value's scale joins its key's
-            // score as a logarithm, so that the weights of the second product,
-            // exp2(x - max) of the joint score, fit in 16 bits whatever the scales
-            // are; the sum of weights takes it out again. A scale of zero counts as
-            // 2^-100 there.
+            // score as a logarithm: the weights of the second product, exp2(x - max) of
+            // the joint score, are relative to what contributes most, and the sum of
+            // weights takes the scale out again. That holds where an element of the row
+            // comes near 448, as kv_cache_write's do. A row of zeros contributes nothing
+            // whatever its scale says, and must not set the maximum: see below. A scale
+            // of zero counts as 2^-100 there.
             float kc[2] = {a.scale, a.scale}, lv[2] = {0.0f, 0.0f}, unscale[2] = {1.0f, 1.0f};
             if constexpr (QUANT) {
                 const float* sc = reinterpret_cast<const float*>(st + 2 * kWarpKeys * ROWB);
@@ -488,11 +505,27 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
 #pragma unroll
                 for (int e = 0; e < 4; ++e) grew |= x[nt][e] > limit[nt][e & 1];
             if (__any_sync(0xffffffffu, grew)) {
+                // Only here, where a maximum is about to move, do values that are all zero matter. Their
+                // weights count in the sum alone; the maximum follows them kEmptyBelow further down, so
+                // that the sum stays finite.
+                uint32_t empty = 0;
+                if constexpr (QUANT) {
+                    constexpr int TIMES = kWarpKeys * CHUNKS / 32;
+                    uint4 w[TIMES];
+#pragma unroll
+                    for (int i = 0; i < TIMES; ++i)
+                        w[i] = *reinterpret_cast<const uint4*>(st + kWarpKeys * ROWB + i * 512 + lane * 16);
+                    empty = empty_rows<CHUNKS>(w) >> g;  // bits 0 and 8: of the lane's keys
+                }
+                auto is_empty = [&](int e) { return QUANT && (empty >> (e >> 1) * 8 & 1) != 0; };
+                auto follow = [&](int nt, int e) {
+                    return is_empty(e) ? x[nt][e] - lv[e >> 1] - kEmptyBelow : x[nt][e];
+                };
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(x[nt][e], x[nt][e + 2]);
+                        float top = fmaxf(follow(nt, e), follow(nt, e + 2));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -509,6 +542,16 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                             }
                         }
                     }
+                if (QUANT && __any_sync(0xffffffffu, (empty & 0x101) != 0)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (is_empty(e)) {
+                                l[nt][e & 1] += ex2(x[nt][e] - lv[e >> 1] - m[nt][e & 1]);
+                                x[nt][e] = -INFINITY;
+                            }
+                }
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)

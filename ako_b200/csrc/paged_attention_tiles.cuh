@@ -90,6 +90,7 @@ struct TilesShape {
 struct TileMeta {
     float kc[kTilesKeys], lv[kTilesKeys], unscale[kTilesKeys];  // of an e4m3 cache, as in the kernel for few rows
     uint32_t there[4];  // keys whose page exists and which some row may see
+    uint32_t empty[4];  // of an e4m3 cache, keys whose values are all zero; known when the values are there
 };
 
 template <int STAGES>
@@ -317,6 +318,34 @@ struct TileLoader {
 __device__ __forceinline__ uint32_t first_bits(int n, int w) {
     const int k = min(max(n - 32 * w, 0), 32);
     return k == 32 ? 0xffffffffu : (1u << k) - 1u;
+}
+
+// Takes the keys whose bits are set in `empty` out of a row's scores x, which hold the logarithms
+// `lv` of their scales: the largest score without those, and the sum of weights relative to it.
+__device__ __forceinline__ void take_out_empty(float (&x)[kTilesKeys], const float* lv, const uint4& empty, float& top,
+                                               float& sum) {
+    const uint32_t bits[4] = {empty.x, empty.y, empty.z, empty.w};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (bits[w] == 0) continue;
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+            if (bits[w] >> c & 1) {
+                x[w * 32 + c] -= lv[w * 32 + c];
+                top = fmaxf(top, x[w * 32 + c]);
+            }
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (bits[w] == 0) continue;
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+            if (bits[w] >> c & 1) {
+                sum += ex2(x[w * 32 + c] - base);
+                x[w * 32 + c] = -INFINITY;
+            }
+    }
 }
 
 template <typename T, bool QUANT, int DPAD>
@@ -579,6 +608,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 mbar_arrive(&sm.k_full[st]);
                 acquire(&sm.v_empty[st], n);
                 if (!ok) break;
+                const uint32_t empty = empty_rows<Loader::CHUNKS>(v);
+                if (lane == 0) sm.meta[n % kMetaStages].empty[warp & 3] = empty;
                 if (load.convert(v, v_tile + st * Shape::kOperand, !now.whole)) sm.odd = 1;
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.v_full[st]);
@@ -731,16 +762,32 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                                 x[w * 32 + c] = (bits & (1u << c)) != 0 ? x[w * 32 + c] : -INFINITY;
                         }
                     }
-                    float tops[4] = {x[0], x[1], x[2], x[3]};
+                    auto largest = [&] {
+                        float tops[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                    for (int c = 4; c < kTilesKeys - 4; c += 8) {
+                        for (int c = 4; c < kTilesKeys - 4; c += 8) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[c + i], x[c + 4 + i]);
-                    }
-                    float top = max3(max3(tops[0], x[124], x[125]), max3(tops[1], x[126], x[127]), fmaxf(tops[2], tops[3]));
-                    top *= scale;
-                    const bool grew = top > ref + (ref == -INFINITY ? 0.0f : kGrowth);
+                            for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], x[c + i], x[c + 4 + i]);
+                        }
+                        return max3(max3(tops[0], x[124], x[125]), max3(tops[1], x[126], x[127]), fmaxf(tops[2], tops[3]));
+                    };
+                    float top = largest() * scale;
+                    auto grows = [&] { return top > ref + (ref == -INFINITY ? 0.0f : kGrowth); };
+                    bool grew = grows();
+                    // Weights of keys whose values are all zero, relative to the largest of them: as in the
+                    // kernel for few rows.
+                    float empty_top = -INFINITY, empty_sum = 0.0f;
                     if (__any_sync(0xffffffffu, grew)) {
+                        if constexpr (QUANT) {
+                            ok = tile_wait(sm, &sm.v_full[n % STAGES], n / STAGES & 1, polls);
+                            ok = __all_sync(0xffffffffu, ok);
+                            const uint4 e4 = *reinterpret_cast<const uint4*>(meta.empty);
+                            if ((e4.x | e4.y | e4.z | e4.w) != 0) {
+                                take_out_empty(x, meta.lv, e4, empty_top, empty_sum);
+                                top = fmaxf(largest(), empty_top - kEmptyBelow);
+                                grew = grows();
+                            }
+                        }
                         const float to = grew ? top : ref;
                         const float alpha = grew ? ex2(ref - to) : 1.0f;
                         ref = to;
@@ -758,6 +805,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                         }
                     }
                     const float base = ref == -INFINITY ? 0.0f : ref;
+                    if (QUANT && empty_sum != 0.0f) sum += empty_sum * ex2(empty_top - base);
                     const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
                     float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
