@@ -9,7 +9,7 @@ from pathlib import Path
 
 import pytest
 import torch
-from paged_oracle import Problem, check_attention, quantise
+from paged_oracle import Problem, attend, check_attention, quantise, sees
 
 from ako_b200 import kv_cache_write_cuda_sm100, paged_attention_cuda_sm100
 
@@ -82,9 +82,11 @@ def test_offsets_far_outside_the_tokens(cuda_device, new) -> None:
     rows that lie between them and no others."""
     p = Problem(torch.bfloat16, False, 10, 2, 64, 16, [(new, new + 30), (new, new + 30), (new, new + 30)], True, 31,
                 cuda_device)
-    want = paged_attention_cuda_sm100(p.q.to(cuda_device), p.kv(), p.batch())
-    check_attention(p, want)
+    check_attention(p, paged_attention_cuda_sm100(p.q.to(cuda_device), p.kv(), p.batch()))
+    # Which keys a CTA takes, and with it the order of the fp32 sums, goes by all sequences' lengths: the last
+    # sequence's rows are held to the bound of such sums and not to the bits of a call with other lengths.
     owned = slice(2 * new, 3 * new)
+    want, bound = attend(p.q[owned], p.k[2], p.v[2], p.v_scale[2], sees(new, new + 30, 0, 0), 64**-0.5, p.dtype, False)
     for cu in ([new, MIN, 2 * new, 3 * new], [MAX, MIN, 2 * new, MAX], [MIN + new, MIN, 2 * new, MAX - 1]):
         # the second sequence holds rows 0 .. 2 * new - 1 where its begin is below 0
         p.cu = torch.tensor(cu, dtype=torch.int32)
@@ -93,7 +95,7 @@ def test_offsets_far_outside_the_tokens(cuda_device, new) -> None:
         if cu[3] > 3 * new:  # the last sequence then owns the two rows behind the others'
             q, out = q[:3 * new], out[:3 * new]
         paged_attention_cuda_sm100(q, p.kv(), p.batch(), out=out)
-        assert torch.equal(out[owned], want[owned])
+        assert bool(((out[owned].double().cpu() - want).abs() <= bound).all())
         assert bool(torch.isfinite(out).all()) and bool((out[3 * new:] == 9).all())
         before = p.caches["k"].clone()
         kv_cache_write_cuda_sm100(p.k_new.to(cuda_device), p.v_new.to(cuda_device), p.kv(), p.batch())
