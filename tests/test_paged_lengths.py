@@ -97,8 +97,9 @@ def test_offsets_far_outside_the_tokens(cuda_device, new) -> None:
         paged_attention_cuda_sm100(q, p.kv(), p.batch(), out=out)
         assert bool(((out[owned].double().cpu() - want).abs() <= bound).all())
         assert bool(torch.isfinite(out).all()) and bool((out[3 * new:] == 9).all())
-        before = p.caches["k"].clone()
+        before = {name: p.caches[name].clone() for name in ("k", "v")}
         kv_cache_write_cuda_sm100(p.k_new.to(cuda_device), p.v_new.to(cuda_device), p.kv(), p.batch())
-        pages = [int(x) for x in p.table[0]]
-        assert torch.equal(p.caches["k"][pages].view(torch.int16), before[pages].view(torch.int16))  # the first has no rows
-        p.caches["k"].copy_(before)
+        pages = [int(x) for x in p.table[0]]  # of the first sequence, which has no rows
+        for name in ("k", "v"):
+            assert torch.equal(p.caches[name][pages].view(torch.int16), before[name][pages].view(torch.int16))
+            p.caches[name].copy_(before[name])
