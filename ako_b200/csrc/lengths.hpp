@@ -5,7 +5,10 @@
 
 namespace ako_b200 {
 
-constexpr int clamp_to(int x, int most) { return x < 0 ? 0 : x < most ? x : most; }
+constexpr int clamp_to(int x, int most) {
+    const int y = x > 0 ? x : 0;
+    return y < most ? y : most;
+}
 
 struct RowRange {
     int first, n;
@@ -15,7 +18,8 @@ struct RowRange {
 // subtracted: begin and end may be any two numbers, and their difference none.
 constexpr RowRange row_range(int begin, int end, int tokens) {
     const int first = clamp_to(begin, tokens), last = clamp_to(end, tokens);
-    return {first, last > first ? last - first : 0};
+    const int n = last - first;
+    return {first, n > 0 ? n : 0};
 }
 
 // Position of new token `at` (0 <= at < n) of a sequence of kv_len tokens, the

@@ -240,12 +240,12 @@ struct PartialBlock {
 // rescaled rarely.
 constexpr float kGrowth = 8.0f;
 
-// A key of an e4m3 cache whose values are all zero, of score s (in powers of
-// two), has a weight and no values: its scale is any number. Rows' maxima, which
-// are those of score + log2(scale), follow such a key as if its scale were 2^-64:
-// its weight is then at most 2^(64 + kGrowth) in the sum, which stays finite, and
-// keys with values keep their 16 bits unless they contribute 2^-64 of it.
-constexpr float kEmptyBelow = 64.0f;
+// What a key of an e4m3 cache whose values are all zero counts with, at most, as the logarithm of its scale, which
+// may be any number (kv_cache_write's is 1). Maxima are those of score + log2(scale), and weights relative to them,
+// so a large scale would take bits from the weights of the keys that do have values. The key's own weight counts in
+// the sum alone: relative to a maximum that follows it 2^64 below, it stays finite there, and is not lost unless it
+// is 2^62 times smaller than that of a key whose scale is 1.
+constexpr float kEmptyLog = -64.0f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

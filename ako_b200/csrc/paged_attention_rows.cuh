@@ -172,8 +172,8 @@ __device__ __forceinline__ void copy_dense(uint32_t to, const uint8_t* from, int
      ...);
 }
 
-// An e4m3 cache's values that are all zero (of either sign): bit r for row r of the 32 / CHUNKS * N
-// rows whose 16-byte chunks a warp holds, lane L chunk L % CHUNKS of rows L / CHUNKS + i * (32 / CHUNKS).
+// An e4m3 cache's rows that are all zero (of either sign): bit r for row r of the 32 / CHUNKS * N rows
+// whose 16-byte chunks a warp holds, lane L chunk L % CHUNKS of the rows L / CHUNKS + i * 32 / CHUNKS.
 template <int CHUNKS, int N>
 __device__ __forceinline__ uint32_t empty_rows(const uint4 (&v)[N]) {
     constexpr int TAKEN = 32 / CHUNKS;
@@ -462,9 +462,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
             // score as a logarithm: the weights of the second product, exp2(x - max) of
             // the joint score, are relative to what contributes most, and the sum of
             // weights takes the scale out again. That holds where an element of the row
-            // comes near 448, as kv_cache_write's do. A row of zeros contributes nothing
-            // whatever its scale says, and must not set the maximum: see below. A scale
-            // of zero counts as 2^-100 there.
+            // comes near 448, as kv_cache_write's do; rows of zeros, which contribute
+            // nothing, count with kEmptyLog below where it would matter. A scale of
+            // zero counts as 2^-100.
             float kc[2] = {a.scale, a.scale}, lv[2] = {0.0f, 0.0f}, unscale[2] = {1.0f, 1.0f};
             if constexpr (QUANT) {
                 const float* sc = reinterpret_cast<const float*>(st + 2 * kWarpKeys * ROWB);
@@ -505,27 +505,31 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
 #pragma unroll
                 for (int e = 0; e < 4; ++e) grew |= x[nt][e] > limit[nt][e & 1];
             if (__any_sync(0xffffffffu, grew)) {
-                // Only here, where a maximum is about to move, do values that are all zero matter. Their
-                // weights count in the sum alone; the maximum follows them kEmptyBelow further down, so
-                // that the sum stays finite.
-                uint32_t empty = 0;
+                // Values that are all zero matter only here, where a maximum is about to move.
                 if constexpr (QUANT) {
                     constexpr int TIMES = kWarpKeys * CHUNKS / 32;
                     uint4 w[TIMES];
 #pragma unroll
                     for (int i = 0; i < TIMES; ++i)
                         w[i] = *reinterpret_cast<const uint4*>(st + kWarpKeys * ROWB + i * 512 + lane * 16);
-                    empty = empty_rows<CHUNKS>(w) >> g;  // bits 0 and 8: of the lane's keys
+                    const uint32_t empty = empty_rows<CHUNKS>(w) >> g;  // bits 0 and 8: of the lane's keys
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if ((empty >> 8 * i & 1) != 0 && lv[i] > kEmptyLog) {
+                            const float by = kEmptyLog - lv[i];
+                            unscale[i] = 0x1p64f;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                x[nt][2 * i] += by;
+                                x[nt][2 * i + 1] += by;
+                            }
+                        }
                 }
-                auto is_empty = [&](int e) { return QUANT && (empty >> (e >> 1) * 8 & 1) != 0; };
-                auto follow = [&](int nt, int e) {
-                    return is_empty(e) ? x[nt][e] - lv[e >> 1] - kEmptyBelow : x[nt][e];
-                };
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(follow(nt, e), follow(nt, e + 2));
+                        float top = fmaxf(x[nt][e], x[nt][e + 2]);
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -542,16 +546,6 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                             }
                         }
                     }
-                if (QUANT && __any_sync(0xffffffffu, (empty & 0x101) != 0)) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (is_empty(e)) {
-                                l[nt][e & 1] += ex2(x[nt][e] - lv[e >> 1] - m[nt][e & 1]);
-                                x[nt][e] = -INFINITY;
-                            }
-                }
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)

@@ -65,8 +65,10 @@ constexpr int kMetaStages = 8;
 constexpr uint32_t kWaitCycles = 1u << 31;  // of a wait, about a second
 constexpr uint32_t kDrainPolls = 1u << 24;
 // Registers per thread of the softmax, loading and issuing warps. The block is
-// launched with 128 a thread, and 2 * 192 + 80 + 48 = 4 * 128.
-constexpr int kSoftmaxRegs = 192, kLoadRegs = 80, kIssueRegs = 48;
+// launched with 128 a thread, and 2 * 192 + 88 + 40 = 4 * 128. An e4m3 cache's
+// loading warps hold a tile's keys or values in them: with 80 and 48, 2048 tokens
+// on 16384 took 863 us where these took 784.
+constexpr int kSoftmaxRegs = 192, kLoadRegs = 88, kIssueRegs = 40;
 
 struct TilesArgs {
     // The cache's keys and values as (page, head, slot, column) in boxes of `box` slots and 64
@@ -318,34 +320,6 @@ struct TileLoader {
 __device__ __forceinline__ uint32_t first_bits(int n, int w) {
     const int k = min(max(n - 32 * w, 0), 32);
     return k == 32 ? 0xffffffffu : (1u << k) - 1u;
-}
-
-// Takes the keys whose bits are set in `empty` out of a row's scores x, which hold the logarithms
-// `lv` of their scales: the largest score without those, and the sum of weights relative to it.
-__device__ __forceinline__ void take_out_empty(float (&x)[kTilesKeys], const float* lv, const uint4& empty, float& top,
-                                               float& sum) {
-    const uint32_t bits[4] = {empty.x, empty.y, empty.z, empty.w};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (bits[w] == 0) continue;
-#pragma unroll
-        for (int c = 0; c < 32; ++c)
-            if (bits[w] >> c & 1) {
-                x[w * 32 + c] -= lv[w * 32 + c];
-                top = fmaxf(top, x[w * 32 + c]);
-            }
-    }
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (bits[w] == 0) continue;
-#pragma unroll
-        for (int c = 0; c < 32; ++c)
-            if (bits[w] >> c & 1) {
-                sum += ex2(x[w * 32 + c] - base);
-                x[w * 32 + c] = -INFINITY;
-            }
-    }
 }
 
 template <typename T, bool QUANT, int DPAD>
@@ -608,8 +582,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                 mbar_arrive(&sm.k_full[st]);
                 acquire(&sm.v_empty[st], n);
                 if (!ok) break;
-                const uint32_t empty = empty_rows<Loader::CHUNKS>(v);
-                if (lane == 0) sm.meta[n % kMetaStages].empty[warp & 3] = empty;
+                const uint32_t empties = empty_rows<Loader::CHUNKS>(v);
+                if (lane == 0) sm.meta[n % kMetaStages].empty[warp & 3] = empties;
                 if (load.convert(v, v_tile + st * Shape::kOperand, !now.whole)) sm.odd = 1;
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.v_full[st]);
@@ -783,8 +757,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                             ok = __all_sync(0xffffffffu, ok);
                             const uint4 e4 = *reinterpret_cast<const uint4*>(meta.empty);
                             if ((e4.x | e4.y | e4.z | e4.w) != 0) {
-                                take_out_empty(x, meta.lv, e4, empty_top, empty_sum);
-                                top = fmaxf(largest(), empty_top - kEmptyBelow);
+#pragma unroll 1
+                                for (int w = 0; w < 4; ++w) {
+#pragma unroll 1
+                                    for (uint32_t bits = meta.empty[w] & meta.there[w]; bits != 0; bits &= bits - 1) {
+                                        const int c = w * 32 + __ffs(bits) - 1;
+                                        __syncwarp();
+                                        const float s = __uint_as_float(tmem_load1(s_at + c)) * (my_factor * meta.kc[c]);
+                                        if (sees_key(a, my_pos, key0 + c) && s != -INFINITY) {
+                                            const float most = fmaxf(empty_top, s);
+                                            empty_sum = empty_sum * ex2(empty_top - most) + ex2(s - most);
+                                            empty_top = most;
+                                        }
+                                    }
+                                }
+                                const uint32_t empty[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+                                for (int c = 0; c < kTilesKeys; ++c)
+                                    if (empty[c / 32] >> (c % 32) & 1) x[c] = -INFINITY;
+                                top = fmaxf(largest(), empty_top + kEmptyLog);
                                 grew = grows();
                             }
                         }
