@@ -235,10 +235,16 @@ struct PartialBlock {
     float o[ROWS][DPAD];
 };
 
-// How far (as a power of two) a row's weights may exceed 1 before what they
-// are relative to is moved: 16-bit weights keep their precision, and sums are
-// rescaled rarely.
+// How far (as a power of two) a row's weights may exceed those that they are
+// relative to before that is moved: 16-bit weights keep their precision, and
+// sums are rescaled rarely.
 constexpr float kGrowth = 8.0f;
+
+// Where the weights' 16-bit type is fp16, which has few exponents, they are taken 2^7 higher: up to
+// 2^15 with kGrowth, of the type's 2^16, so that a weight keeps all its bits down to 2^-21 of the
+// largest, and some down to 2^-31. The sums take the factor along, and their quotient drops it.
+template <typename M>
+constexpr float kLift = std::is_same_v<M, __half> ? 7.0f : 0.0f;
 
 // What a key of an e4m3 cache whose values are all zero counts with, at most, as the logarithm of its scale, which
 // may be any number (kv_cache_write's is 1). Maxima are those of score + log2(scale), and weights relative to them,

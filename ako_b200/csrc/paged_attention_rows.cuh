@@ -535,8 +535,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                         if (top > limit[nt][e]) {
                             // nothing has been summed yet where there was no limit
-                            const float alpha = limit[nt][e] == -INFINITY ? 0.0f : ex2(m[nt][e] - top);
-                            m[nt][e] = top;
+                            const float to = top - kLift<M>;
+                            const float alpha = limit[nt][e] == -INFINITY ? 0.0f : ex2(m[nt][e] - to);
+                            m[nt][e] = to;
                             limit[nt][e] = top + kGrowth;
                             l[nt][e] *= alpha;
 #pragma unroll

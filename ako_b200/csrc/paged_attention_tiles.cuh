@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                             }
                         }
                     }
-                    const float base = ref == -INFINITY ? 0.0f : ref;
+                    const float base = ref == -INFINITY ? 0.0f : ref - kLift<M>;
                     if (QUANT && empty_sum != 0.0f) sum += empty_sum * ex2(empty_top - base);
                     const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
                     float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
