@@ -480,7 +480,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsShape<T, QUANT, DPAD, NT>::
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if constexpr (QUANT) x[nt][e] = fmaf(x[nt][e] * factor[nt][e & 1], kc[e >> 1], lv[e >> 1]);
+                    // the powers of two of q's row and of the key first: one may be as large as the other is small
+                    if constexpr (QUANT) x[nt][e] = fmaf(x[nt][e], factor[nt][e & 1] * kc[e >> 1], lv[e >> 1]);
                     else x[nt][e] *= a.scale;
                 }
             const bool whole = there == 0xffffu && key0 + kWarpKeys - 1 <= it.p_lo &&
