@@ -427,6 +427,11 @@ bool make_rows(const void* p, int64_t sb, int64_t nb, int64_t ss, int64_t ns, in
     return aligned16(p);
 }
 
+// Whether places of a cache's tensor are one place: which write is left there would be chance.
+bool repeats(const PagedTensor& t, const PagedCache& c) {
+    return (c.num_pages > 1 && t.page == 0) || (c.kv_heads > 1 && t.head == 0) || (c.page_size > 1 && t.slot == 0);
+}
+
 // Pointer and the strides of axes longer than one are multiples of 16 bytes.
 bool rows16(const void* p, int64_t s0, int64_t n0, int64_t s1, int64_t n1, int64_t s2, int64_t n2, int es) {
     return aligned16(p) && multiple16(s0, n0, es) && multiple16(s1, n1, es) && multiple16(s2, n2, es);
@@ -454,6 +459,11 @@ extern "C" int ako_b200_kv_cache_write(const void* k, int64_t k_stride_b, int64_
         return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: tokens * kv_heads must be < 2^31", op);
     if (k == nullptr || v == nullptr)
         return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: k or v is a null pointer", op);
+    const bool quant = cache->dtype == AKO_B200_E4M3;
+    if (repeats(a.cache.k, a.cache) || repeats(a.cache.v, a.cache) ||
+        (quant && (repeats(a.cache.ks, a.cache) || repeats(a.cache.vs, a.cache))))
+        return set_error(AKO_B200_ERR_INVALID_ARGUMENT, "%s: a cache that repeats its elements along an axis (a stride "
+                                                        "of 0) cannot be written", op);
     const bool uniform = a.seqs.cu == nullptr;
     const int64_t nb = uniform ? a.seqs.batch : 1, ns = uniform ? q_len : tokens;
     const int in = dtype_size(dtype);
@@ -465,7 +475,6 @@ extern "C" int ako_b200_kv_cache_write(const void* k, int64_t k_stride_b, int64_
     a.heads = FastDiv::make(static_cast<uint32_t>(a.cache.kv_heads));
     a.rows = static_cast<uint32_t>(tokens * a.cache.kv_heads);
     a.q_len = FastDiv::make(static_cast<uint32_t>(uniform ? q_len : 1));
-    const bool quant = cache->dtype == AKO_B200_E4M3;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
         case AKO_B200_F32: return launch_write<float>(a, quant, st);

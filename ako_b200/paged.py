@@ -211,7 +211,7 @@ def kv_cache_write_cuda_sm100(k: torch.Tensor, v: torch.Tensor, cache: PagedKV, 
     any of the three activation dtypes for a quantised cache, which takes
     ``round(x / s)`` under the least power of two ``s`` that keeps the token's
     values of a head within e4m3's 448, and stores ``s`` with it. Tokens of one
-    call must not share a slot.
+    call must not share a slot; a cache expanded along an axis is refused.
     """
     fn = "kv_cache_write_cuda_sm100"
     _require_cuda(k, fn)

@@ -304,7 +304,8 @@ typedef struct {
  * contiguous. A token at a position before 0 (a sequence of fewer cached than
  * new tokens) is not stored, nor is one at a position past the table (a length
  * that the table does not hold): no token takes an earlier one's place. No two
- * tokens of a call may share a slot.
+ * tokens of a call may share a slot, and a cache whose strides are 0 along an
+ * axis of more than one, which can be read, is refused.
  *
  * An e4m3 cache takes round(x / s) to nearest even, where s, the scale stored
  * with it, is the least power of two with max|x| / s <= 448 over the token's
