@@ -37,7 +37,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from ako_b200 import _native, kernels
-from ako_b200.paged import (PagedBatch, PagedKV, kv_cache_write_cuda_sm100,
+from ako_b200.paged import (E4M3, PagedBatch, PagedKV, kv_cache_write_cuda_sm100,
                             paged_attention_cuda_sm100)
 from ako_b200.reference import ops as reference_ops
 
@@ -106,6 +106,13 @@ class PagedKVCache:
                  kv_dtype: torch.dtype | None = None, window: int = 0, sinks: int = 0) -> None:
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"PagedKVCache: attention over pages supports float16/bfloat16 models, got {dtype}")
+        if page_size < 1 or max_len < 1 or batch < 1:
+            raise ValueError(f"PagedKVCache: batch, max_len and page_size must be >= 1, got {batch}, {max_len} and "
+                             f"{page_size}")
+        if kv_dtype not in (None, dtype, E4M3):
+            raise ValueError(f"PagedKVCache: keys and values are kept as {dtype} or {E4M3}, got {kv_dtype}")
+        if window < 0 or sinks < 0:
+            raise ValueError(f"PagedKVCache: window and sinks must be >= 0, got {window} and {sinks}")
         pages = -(-max_len // page_size)
         self.layers = [PagedKV.empty(batch * pages, config.n_kv_heads, page_size, config.head_dim,
                                      dtype=kv_dtype or dtype, device=device) for _ in range(config.n_layers)]

@@ -4,7 +4,11 @@ dereferenced, and in Python."""
 from __future__ import annotations
 
 import pytest
+import torch
 from test_paged import E4M3_CODE, P, cache, lib, read, seqs, write  # noqa: F401
+from test_paged_decoder import SMALL
+
+from ako_b200.decoder import ModelConfig, PagedKVCache
 
 
 @pytest.mark.parametrize("stride", ["page", "head", "slot"])
@@ -22,3 +26,14 @@ def test_a_cache_that_repeats_its_elements_is_not_written(lib, tensor, stride) -
     # reading such a cache is allowed: the next refusal is another's
     assert read(lib, cache(**{**scales, f"{tensor}_stride_{stride}": 0}), seqs(), k=None) == 1
     assert b"k_out or v_out is a null pointer" in lib.ako_b200_last_error()
+
+
+@pytest.mark.parametrize("what,words", [
+    ({"page_size": 0}, "page_size must be >= 1"), ({"page_size": -16}, "page_size must be >= 1"),
+    ({"max_len": 0}, "max_len"), ({"batch": 0}, "batch"), ({"kv_dtype": torch.float32}, "kept as"),
+    ({"kv_dtype": torch.float16}, "kept as"), ({"window": -1}, "window"), ({"sinks": -1}, "sinks")])
+def test_a_paged_cache_of_the_decoder_that_could_not_be_used(what, words) -> None:
+    """Refused when it is made, and not as a division by zero or at the first step."""
+    made = {"batch": 2, "max_len": 16, "device": "cpu", "dtype": torch.bfloat16, **what}
+    with pytest.raises(ValueError, match=words):
+        PagedKVCache(ModelConfig(**SMALL), **made)
