@@ -75,8 +75,10 @@ class PagedKV:
     page_size, kv_heads, head_dim)`` is passed as its ``transpose(1, 2)``),
     all on 16-byte boundaries. ``k_scale`` and ``v_scale``: float32
     ``(num_pages, kv_heads, page_size)``, for a quantised cache only; a cached
-    value stands for ``element * scale``, scales being positive (attention takes
-    a value's below 2^-100 for that). ``head_dim`` is a multiple of 8 (16
+    value stands for ``element * scale``, scales being positive. Attention takes
+    a value's scale below 2^-100 for that, and those of the keys that a row sees
+    should lie within 2^100 of one another: past 2^126 a key of the smaller ones
+    is lost from the row's sum of weights. ``head_dim`` is a multiple of 8 (16
     when quantised) up to 128; attention takes float16 and bfloat16 queries.
     """
 
@@ -134,8 +136,11 @@ class PagedBatch:
     the same number, or, with ``cu_seqlens`` (int32 ``(batch + 1,)``),
     ``(tokens, heads, head_dim)`` in which sequence ``b`` owns the rows
     ``cu_seqlens[b]`` up to ``cu_seqlens[b + 1]``. ``max_q_len``: most new
-    tokens of a sequence where ``cu_seqlens`` is given, for the choice of a
-    kernel only (default: all of the call's).
+    tokens of a sequence where ``cu_seqlens`` is given, for attention's choice of
+    a kernel only. Without it that takes all of the call's tokens for those of
+    one sequence, and a step of single tokens runs on the kernel for chunks: 69
+    us in place of 47 for 32 sequences of 1500 to 2176 tokens (32 heads of 128, 8
+    kv heads, bfloat16), 141 in place of 38 with an e4m3 cache.
 
     No call reads these tensors on the host. What they say is clamped to what
     there is: lengths to the table and to the tokens given; a page number

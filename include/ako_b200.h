@@ -255,9 +255,16 @@ int ako_b200_swiglu_plan(int64_t n_rows, int64_t hidden_dim, int dtype, int alig
  * with free element strides for the first three axes; the last is contiguous.
  * dtype is that of the activations, or AKO_B200_E4M3 with one fp32 scale per
  * token and head in k_scale and v_scale, (num_pages, kv_heads, page_size) with
- * free strides: a cached value stands for element * scale. Scales are
- * positive; attention takes a v_scale below 2^-100 for that. k, v and all their strides are multiples of 16 bytes, head_dim a
- * multiple of 8 (of 16 in an e4m3 cache) and at most 128.
+ * free strides: a cached value stands for element * scale. k, v and all their
+ * strides are multiples of 16 bytes, head_dim a multiple of 8 (of 16 in an e4m3
+ * cache) and at most 128.
+ *
+ * Scales are positive. Attention takes a v_scale below 2^-100 for that, and one
+ * above 2^-64 for that where it would matter and the values are all zero. The
+ * v_scales of the keys that a row sees should lie within 2^100 of one another:
+ * the sum of weights is kept in fp32 relative to the largest weight * v_scale, so
+ * that a key whose v_scale is 2^-d of that one's is lost from the sum where its
+ * weight is below 2^(d - 126) of it.
  */
 typedef struct {
     void* k;
@@ -340,7 +347,9 @@ int ako_b200_kv_cache_read(const ako_b200_paged_kv* cache, const ako_b200_paged_
  * q and out are laid out as ako_b200_kv_cache_write's k and v, with q_heads
  * heads, in fp16 or bf16 (`dtype`). Scores, the softmax's maximum and sum and
  * the output's sum are fp32; the weights are rounded to the operands' 16-bit
- * type for the second product, the output once.
+ * type for the second product (fp16 for an e4m3 cache), the output once. In fp16
+ * a weight keeps all its bits down to 2^-21 of the row's largest (weight *
+ * v_scale in an e4m3 cache), and some down to 2^-31.
  *
  * workspace: device memory of at least the bytes that
  * ako_b200_paged_attention_plan reports, 16-byte aligned, used by this call
