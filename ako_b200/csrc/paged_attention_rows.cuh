@@ -13,10 +13,10 @@
 //
 // Bound: HBM, by the keys and values read once. 32 contexts of 2048 tokens (32
 // heads of 128, 8 kv heads, bf16, 252 MB): 48 us, 5.2 TB/s with the launch's
-// begin and end; 16 e4m3 contexts of 2000 to 65536 tokens (849 MB): 149 us,
-// 5.7 TB/s. Instructions count for almost as much: addresses made of constants
-// took those two from 51 and 157 us (the latter, at the clock of a long run,
-// from 169).
+// begin and end; 16 e4m3 contexts of 2000 to 65536 tokens (849 MB): 149 to 159
+// us by the card, 5.7 to 5.3 TB/s. Instructions count for almost as much:
+// addresses made of constants took those two from 51 and 157 us (the latter, at
+// the clock of a long run, from 169).
 #pragma once
 
 #include <utility>

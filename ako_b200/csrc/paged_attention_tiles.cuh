@@ -26,7 +26,8 @@
 // rescaled rarely.
 //
 // Where items change, what the next one needs is found while the last products
-// run, and that code is kept short (8 prompts of 2048 tokens: 382 to 347 us).
+// run, and that code is kept short: it took 8 prompts of 2048 tokens from 382 to
+// 347 us on one card. Over the cards and clocks met they take 345 to 397 us.
 //
 // Bound: per tile and half, two products of 128 x 128 x head_dim take 8 *
 // head_dim cycles and the 16384 exponentials 1024 cycles of the SM's 16 a
@@ -34,10 +35,15 @@
 // halves. Measured, a tile takes about 3500: a half's softmax (2000 from the
 // scores' arrival to the last weights) and its products do not overlap, and
 // the halves' products wait for one another. 2048 new tokens on 16384 cached
-// ones, 32 heads of 128 and 8 kv heads: 498 us in bf16, 1.17 PFLOP/s; 851 us in
-// e4m3, where the softmax reads three more numbers for each key from shared
-// memory and four warps convert every tile through registers. (Fetching values
-// while keys are converted made no difference: 865 us.)
+// ones, 32 heads of 128 and 8 kv heads: 498 to 585 us in bf16 by the card and its
+// clock, 1.17 to 1.00 PFLOP/s; 826 to 841 us in e4m3 (786 to 796 with fp16
+// queries), where the softmax reads three more numbers for each key from shared
+// memory and four warps convert every tile through registers.
+//
+// A key of an e4m3 cache whose values are all zero must not set a row's maximum
+// (kEmptyLog). The loading warps note such keys with the values, and the softmax
+// waits for that where a maximum is about to move, once or a few times an item:
+// 83 to 87 us for 12 mixed sequences, 650 to 670 for e4m3 prompts of 8 x 2048.
 //
 // Every wait is bounded. If one runs out, all roles stop waiting, the rows not
 // yet written become NaN, and the status word is set.
