@@ -1,5 +1,5 @@
-"""Calls of attention from several host threads at once, each on a stream of its own, the first of the process among
-them."""
+"""The first calls of attention in a process: from several host threads at once, each on a stream of its own, and while
+a graph is captured. Each test runs a process of its own, so that nothing that a launch remembers is there yet."""
 
 from __future__ import annotations
 
@@ -47,9 +47,32 @@ print("equal")
 """
 
 
+CAPTURED = """
+import sys
+sys.path[:0] = [{repo!r}, {tests!r}]
+import torch
+from paged_oracle import Problem, check_attention
+from ako_b200 import paged_attention_cuda_sm100
+
+dev = torch.device("cuda", 0)
+for new in (90, 1):
+    for quantised in (False, True):
+        p = Problem(torch.bfloat16, quantised, 8, 2, 128, 16, [(new, 300), (new, 100)], False, 1, dev)
+        q, cache, batch = p.q.to(dev), p.kv(), p.batch()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged_attention_cuda_sm100(q, cache, batch)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(p, out)
+print("equal")
+"""
+
+
 @pytest.mark.gpu
-def test_first_calls_from_eight_threads(cuda_device) -> None:
-    """In a process of its own, so that nothing that a launch remembers is there yet."""
-    got = subprocess.run([sys.executable, "-c", CODE.format(repo=str(REPO), tests=str(REPO / "tests"))],
+@pytest.mark.parametrize("code", [CODE, CAPTURED], ids=["threads", "captured"])
+def test_first_calls_of_a_process(cuda_device, code) -> None:
+    got = subprocess.run([sys.executable, "-c", code.format(repo=str(REPO), tests=str(REPO / "tests"))],
                          capture_output=True, text=True, timeout=300)
     assert got.returncode == 0 and "equal" in got.stdout, got.stderr[-3000:]
