@@ -763,6 +763,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attn_tiles_kernel(const __gr
                             ok = __all_sync(0xffffffffu, ok);
                             const uint4 e4 = *reinterpret_cast<const uint4*>(meta.empty);
                             if ((e4.x | e4.y | e4.z | e4.w) != 0) {
+                                // Few keys: read again from tensor memory one by one. Code for any of the 128
+                                // registers would take more of them from every tile (fp16 queries, 2048 tokens on
+                                // 16384: 805 us, and 788 so).
 #pragma unroll 1
                                 for (int w = 0; w < 4; ++w) {
 #pragma unroll 1

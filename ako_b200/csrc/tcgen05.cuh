@@ -53,11 +53,16 @@ __device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t* r) {
         : "r"(at));
 }
 
+// One column, waited for.
 __device__ __forceinline__ uint32_t tmem_load1(uint32_t at) {
     uint32_t r;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(at) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r)
+                 : "r"(at)
+                 : "memory");
     return r;
 }
+
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
